@@ -15,6 +15,7 @@
  *   llmgen_decode_buckets     src/executor.zig:609-632      (captureGraphs bucket sizes)
  *   llmgen_plan_passes        src/executor.zig:986-1043     (execute: passes of <= max_tokens, flushPass)
  *   llmgen_graphs_*           src/executor.zig:530-575, 609-660 (forward's bucket replay, captureGraphs)
+ *   llmgen_blocks_*           src/runner/block.zig (BlockManager), with shared pages
  * Conventions: host pointers unless named *_dev; bf16 as uint16_t bits; launches on the library stream
  * (include/llmgen_attn.h).  Functions returning int return 0 on success and a negative value on bad arguments.
  */
@@ -99,6 +100,45 @@ void llmgen_bind_step(llmgen_step_state *st, void *meta_dev, llmgen_layout lay, 
  * Decode steps issue store_kv and decode as one launch (hip_attn_decode_store_kv). */
 int llmgen_paged_attention(const llmgen_step_state *st, uint16_t *out, const uint16_t *q, const uint16_t *k,
                            const uint16_t *v, uint16_t *k_cache, uint16_t *v_cache, int store_kv);
+
+/* A layer's form of the cache other than bf16 pages of which every key is seen (include/llmgen_cache.h): pages held in
+ * 4 bits (kv4 != 0), a sliding window and sinks (window 0: none), and the scratch its launches share (may be NULL). */
+typedef struct llmgen_cache_form {
+    int32_t kv4, window, sinks;
+    void *work;
+    size_t work_bytes;
+} llmgen_cache_form;
+
+/* llmgen_paged_attention for such a layer: hip_store_kv4 or hip_store_kv of the step's k / v (unless store_kv == 0),
+ * then hip_attn_decode_* or hip_attn_prefill_*.  form NULL, or one of bf16 pages without a window, is
+ * llmgen_paged_attention.  No reference counterpart. */
+int llmgen_paged_attention_form(const llmgen_step_state *st, const llmgen_cache_form *form, uint16_t *out,
+                                const uint16_t *q, const uint16_t *k, const uint16_t *v, void *k_cache, void *v_cache,
+                                int store_kv);
+
+/* A block manager with reference counts, so that sequences can share pages: the reference's free stack
+ * (src/runner/block.zig) gives a page to one sequence only.  Host state; not thread-safe.  Ids lie in
+ * [0, num_blocks).  Every function that takes a table checks it first and changes nothing if it is refused (-1). */
+void *llmgen_blocks_create(int num_blocks);
+void llmgen_blocks_destroy(void *blocks);
+int llmgen_blocks_free_count(const void *blocks);
+int llmgen_blocks_ref(const void *blocks, int id); /* sequences that hold page id; -1 for a bad id */
+/* n pages for one sequence, the lowest free ids first; -1 if fewer than n are free. */
+int llmgen_blocks_alloc(void *blocks, int n, int32_t *out);
+/* One more sequence shares the pages of a table. */
+int llmgen_blocks_fork(void *blocks, const int32_t *table, int n);
+/* One sequence less holds them; pages that nobody holds are free.  Entries below 0 (already given back, as those a
+ * window has passed) are skipped. */
+int llmgen_blocks_free(void *blocks, const int32_t *table, int n);
+/* Before a write into table[idx]: 0 if this sequence alone holds the page; 1 if others share it: the table then has a
+ * page of its own in its place, and *src / *dst name the copy to make (hip_copy_blocks); -1 if no page is free. */
+int llmgen_blocks_writable(void *blocks, int32_t *table, int idx, int32_t *src, int32_t *dst);
+/* Moves the pages in use to the lowest ids: the copies to make go to src / dst (room for cap pairs; at least free
+ * pages below the highest used one), their number is returned (-1: more than cap, nothing moved).  Every table must then
+ * be passed to llmgen_blocks_remap. */
+int llmgen_blocks_compact(void *blocks, int32_t *src, int32_t *dst, int cap);
+/* Replaces src[i] by dst[i] in a table (entries below 0 stay).  0, or -1 on bad arguments. */
+int llmgen_blocks_remap(int32_t *table, int n, const int32_t *src, const int32_t *dst, int n_pairs);
 
 int llmgen_part_size(int n_seq);
 int llmgen_max_parts(int n_seq, size_t max_model_len);

@@ -1,4 +1,5 @@
-"""ctypes binding of libllmgen_attn.so (the C-ABI declared in include/llmgen_attn.h and include/llmgen_model.h).
+"""ctypes binding of libllmgen_attn.so (the C-ABI declared in include/llmgen_attn.h, include/llmgen_model.h and
+include/llmgen_cache.h).
 
 The library is loaded from the package directory (built in-tree by ``llmgen_amd.build``).  There is no fallback:
 if the library is missing or fails to load, :func:`lib` raises, so nothing on the product path can silently run
@@ -17,7 +18,7 @@ _F = ctypes.c_float
 _SZ = ctypes.c_size_t
 _L = ctypes.c_long
 
-# name -> (restype, argtypes); must match include/llmgen_attn.h and include/llmgen_model.h
+# name -> (restype, argtypes); must match include/llmgen_attn.h, include/llmgen_model.h and include/llmgen_cache.h
 SIGNATURES = {
     "hip_store_kv": (None, [_P, _P, _P, _P, _P, _I, _I, _I, _I]),
     "hip_attn_decode": (None, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _I, _I]),
@@ -69,6 +70,17 @@ SIGNATURES = {
     "hip_sample": (None, [_P, _P, _P, _P, _I, _I, _P]),
     "hip_sample_scratch_bytes": (_SZ, [_I]),
     "hip_qk_norm_rope_store_kv": (None, [_P, _P, _P, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _I, _I, _I, _I, _I]),
+    # include/llmgen_cache.h
+    "hip_kv4_block_bytes": (_SZ, [_I, _I, _I]),
+    "hip_store_kv4": (None, [_P, _P, _P, _P, _P, _I, _I, _I, _I]),
+    "hip_load_kv4": (None, [_P, _P, _P, _P, _P, _I, _I, _I, _I]),
+    "hip_attn_work_bytes": (_SZ, []),
+    "hip_attn_work_init": (None, [_P, _SZ]),
+    "hip_attn_decode_window": (None, [_P] * 6 + [_I] * 6 + [_F, _I, _I, _I, _P, _SZ]),
+    "hip_attn_decode_kv4": (None, [_P] * 6 + [_I] * 6 + [_F, _I, _I, _I, _P, _SZ]),
+    "hip_attn_prefill_window": (None, [_P] * 9 + [_I] * 6 + [_F, _I, _I, _I, _P, _SZ]),
+    "hip_attn_prefill_kv4": (None, [_P] * 9 + [_I] * 6 + [_F, _I, _I, _I, _P, _SZ]),
+    "hip_copy_blocks": (None, [_P, _I, _SZ, _I, _P, _P, _I]),
 }
 
 _lib = None

@@ -29,6 +29,7 @@ import torch
 from . import host as H
 from . import step as stepmod
 from ._lib import lib
+from .cache import kv4_pool
 
 
 class AttentionNeedsBf16(TypeError):
@@ -49,10 +50,13 @@ g_step = H.StepState()  # the bound step (C++ llmgen_step_state)
 @dataclass
 class LayerState:
     """memory/page_atten.zig:15-28: one contiguous K pool and one V pool of
-    num_blocks x [nkv][block_size][hd] bf16 per layer."""
+    num_blocks x [nkv][block_size][hd] bf16 per layer.  ``form``: another form of the cache (4-bit pages, a sliding
+    window), with the scratch of its launches in ``work``."""
 
     k: torch.Tensor
     v: torch.Tensor
+    form: Optional["H.CacheForm"] = None
+    work: Optional[torch.Tensor] = None
 
 
 @dataclass
@@ -60,10 +64,23 @@ class PagedAttentionManager:
     layers: Dict[int, LayerState] = field(default_factory=dict)
 
     def reserve_layer(self, layer_id: int, num_blocks: int, nkv: int, block_size: int, hd: int,
-                      device="cuda") -> LayerState:
-        shape = (num_blocks, nkv, block_size, hd)
-        st = LayerState(torch.zeros(shape, dtype=torch.bfloat16, device=device),
-                        torch.zeros(shape, dtype=torch.bfloat16, device=device))
+                      device="cuda", kv4: bool = False, window: int = 0, sinks: int = 0,
+                      work: Optional[torch.Tensor] = None) -> LayerState:
+        """``kv4``: the pages are held in 4 bits; ``window`` > 0: rows see the last ``window`` keys and the first
+        ``sinks`` ones (include/llmgen_cache.h).  Layers of one stream share a ``work`` buffer (cache.attn_work),
+        without which long sequences are not split."""
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks must not be negative")
+        if kv4:
+            pools = [kv4_pool(num_blocks, nkv, block_size, hd, device) for _ in range(2)]
+        else:
+            shape = (num_blocks, nkv, block_size, hd)
+            pools = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(2)]
+        st = LayerState(*pools)
+        if kv4 or window:
+            st.work = work
+            st.form = H.CacheForm(int(kv4), window, sinks, None if work is None else work.data_ptr(),
+                                  0 if work is None else work.numel() * work.element_size())
         self.layers[layer_id] = st
         return st
 
@@ -118,8 +135,11 @@ class PagedAttentionImpl:
         q, k, v = out.src
         for t in (out.data, q, kv.k, kv.v) + ((k, v) if store_kv else ()):
             _ptr(t)
-        H.paged_attention(g_step, out.data, q, k if store_kv else None, v if store_kv else None, kv.k, kv.v,
-                          store_kv=store_kv)
+        k, v = (k, v) if store_kv else (None, None)
+        if kv.form is None:
+            H.paged_attention(g_step, out.data, q, k, v, kv.k, kv.v, store_kv=store_kv)
+        else:
+            H.paged_attention_form(g_step, kv.form, out.data, q, k, v, kv.k, kv.v, store_kv=store_kv)
 
 
 # attention_v1.zig:123: the legacy FLASH_ATTN node runs the same implementation

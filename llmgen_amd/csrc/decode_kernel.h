@@ -48,7 +48,12 @@ struct DecodeLds {
 // The split-K decode workgroup's work, as a device function so that other kernels can run it as one of their
 // workgroup roles.  (bx, by, bz) play the part of the grid position (kv head, sequence or list entry, span);
 // n_list is the length of the tile list in a prefill-metadata launch; lds holds a DecodeLds<G, NT, W>.
-template <int G, int NT, bool POW2, bool FUSE, int W>
+// WIN: the row sees only the last `window` keys and the first `sinks` ones.  Spans and rounds then run over the visible
+// keys: the sinks, padded to a multiple of a wave's tokens so that no wave's tokens lie on both sides of the gap, then
+// the window from its first key down to a multiple of 4 (the four rows of a DMA instruction keep one page).  The padding
+// is masked, and reads visible rows in its place.  span must be a multiple of NT * 16; a sequence with more visible keys
+// than nparts spans hold takes longer ones.
+template <int G, int NT, bool POW2, bool FUSE, int W, bool WIN = false>
 __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, float *__restrict__ part_o, float *__restrict__ part_ml,
                              const bf16_t *__restrict__ q, const bf16_t *__restrict__ kc,
                              const bf16_t *__restrict__ vc, const int *__restrict__ block_tables,
@@ -57,7 +62,9 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
                              int *__restrict__ counters, const int *__restrict__ cu_q,
                              const int *__restrict__ tile_seq, const bf16_t *__restrict__ k_new,
                              const bf16_t *__restrict__ v_new, const int *__restrict__ slots,
-                             bf16_t *__restrict__ kc_w, bf16_t *__restrict__ vc_w, int bx, int by, int bz, int n_list, unsigned char *lds) {
+                             bf16_t *__restrict__ kc_w, bf16_t *__restrict__ vc_w, int bx, int by, int bz, int n_list, unsigned char *lds,
+                             int window = 0, int sinks = 0) {
+    static_assert(!(WIN && FUSE), "the fused write knows the whole context only");
     constexpr int WTOK = NT * 16;              // tokens per wave per round
     constexpr int RTOK = W * WTOK;             // tokens per round
     constexpr int NTH = 64 * W;
@@ -72,7 +79,26 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
         row = cu_q[s];
         if (cu_q[s + 1] - row != 1) return;
     }
-    const int ctx = ctx_lens[s];
+    const int ctx_all = WIN ? (int)min((long)ctx_lens[s], (long)max_blocks * block_size) : ctx_lens[s];
+    // WIN: visible keys [0, n_sink) and [lo, ctx_all); the window part starts at index n_sink_pad, for key lo4
+    int lo = 0, lo4 = 0, n_sink = 0, n_sink_pad = 0;
+    if constexpr (WIN) {
+        lo = max(0, ctx_all - window);
+        if (sinks >= lo) lo = 0;  // nothing lies between the sinks and the window
+        else n_sink = sinks;
+        lo4 = lo & ~3;
+        n_sink_pad = (n_sink + WTOK - 1) / WTOK * WTOK;
+    }
+    const int ctx = WIN && ctx_all > 0 ? n_sink_pad + ctx_all - lo4 : ctx_all;  // keys to walk
+    if constexpr (WIN) span = max(span, ((ctx + nparts - 1) / nparts + WTOK - 1) / WTOK * WTOK);
+    auto token = [&](int i) {  // key at index i of the walk (a visible one in place of padding)
+        if constexpr (!WIN) return i;
+        else return i < n_sink_pad ? min(i, n_sink - 1) : max(i - n_sink_pad + lo4, lo);
+    };
+    auto visible = [&](int i) {
+        if constexpr (!WIN) return true;
+        else return i < n_sink_pad ? i < n_sink : i - n_sink_pad + lo4 >= lo;
+    };
     const int t0 = part * span;
     // Fused KV write (decode launch only): this step's token sits at position ctx - 1.  Part 0 copies its K/V
     // rows into the cache slot; the workgroup whose span holds position ctx - 1 reads them from k_new / v_new,
@@ -163,15 +189,15 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
         const int wbase = r * RTOK + wave * WTOK;
         int vt[4 * NT], vblk[4 * NT];
 #pragma unroll
-        for (int j = 0; j < 4 * NT; ++j) vt[j] = t0 + min(wbase + rgrp + 4 * j, n - 1);
+        for (int j = 0; j < 4 * NT; ++j) vt[j] = token(t0 + min(wbase + rgrp + 4 * j, n - 1));
 #pragma unroll
         for (int j = 0; j < 4 * NT; ++j) vt_keep[j] = vt[j];
         if (fuse) b.knew = ld16(k_new + new_row + col * 8);  // issued before the K rows: covered by their wait
         if (SCAL) {
             // the wave's WTOK tokens touch at most two blocks: two scalar block-table reads (scalar cache,
             // their own wait counter), then a per-lane select
-            const int b0 = __builtin_amdgcn_readfirstlane((t0 + min(wbase, n - 1)) >> bs_shift);
-            const int b1 = __builtin_amdgcn_readfirstlane((t0 + min(wbase + WTOK - 1, n - 1)) >> bs_shift);
+            const int b0 = __builtin_amdgcn_readfirstlane(token(t0 + min(wbase, n - 1)) >> bs_shift);
+            const int b1 = __builtin_amdgcn_readfirstlane(token(t0 + min(wbase + WTOK - 1, n - 1)) >> bs_shift);
             const int p0 = bt[b0], p1 = bt[b1];
 #pragma unroll
             for (int j = 0; j < 4 * NT; ++j) vblk[j] = (vt[j] >> bs_shift) == b0 ? p0 : p1;
@@ -194,7 +220,7 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
 #pragma unroll
             for (int j = 0; j < 4 * NT; ++j) {
                 const int kch = col ^ ((rgrp + 4 * j) & 15);
-                const int u = t0 + min(wb + 4 * j, n - 1);  // the instruction's first row (wave-uniform)
+                const int u = token(t0 + min(wb + 4 * j, n - 1));  // the instruction's first row (wave-uniform)
                 const int voff = ((vt[j] & (block_size - 1)) * HD + kch * 8) * 2;
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     (u >> bs_shift) == kb0_blk ? krs0 : krs1,
@@ -227,6 +253,13 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
 
     auto compute = [&](int r, const Buf &b) {
         const int wbase = r * RTOK + wave * WTOK;
+        auto v_row = [&](int j) {  // WIN: rows read in place of padding count for nothing, infinities among them
+            if constexpr (WIN) {
+                const int i = wbase + rgrp + 4 * j;
+                if (i >= n || !visible(t0 + i)) return u32x4_t{0, 0, 0, 0};
+            }
+            return b.vf[j];
+        };
         // ---- this wave's K rows in its LDS slice, then the MFMA B fragments out of it (tile tau, chunk c =
         //      dims c*32 + rgrp*8 of token tau*16 + col); the XOR swizzle keeps both directions conflict-free ----
         // vmcnt(4 NT): the K rows (issued before the 4 NT V loads) have landed
@@ -258,7 +291,7 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
             for (int c = 0; c < 4; ++c)
                 acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qa[c], __builtin_bit_cast(bf16x8_t, kf[tau][c]),
                                                               acc, 0, 0, 0);
-            const bool valid = wbase + tau * 16 + col < n;
+            const bool valid = wbase + tau * 16 + col < n && visible(t0 + wbase + tau * 16 + col);
 #pragma unroll
             for (int i = 0; i < 4; ++i) sc[tau][i] = valid ? acc[i] * scale_log2 : -INFINITY;
         }
@@ -300,7 +333,7 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
 #pragma unroll
             for (int j = 0; j < 4 * NT; ++j) {
                 const int t = rgrp + 4 * j;
-                k_lds[wave][t][col ^ ((t << 2) & 15)] = b.vf[j];
+                k_lds[wave][t][col ^ ((t << 2) & 15)] = v_row(j);
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -357,7 +390,7 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
 #pragma unroll
         for (int j = 0; j < 4 * NT; ++j) {
             float f[8];
-            unpack_bf16x8(b.vf[j], f);
+            unpack_bf16x8(v_row(j), f);
             const float *pp = p_lds[wave][rgrp + 4 * j];
 #pragma unroll
             for (int g = 0; g < G; ++g) {

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "llmgen_attn.h"
+#include "llmgen_cache.h"
 #include "llmgen_host.h"
 #include "llmgen_model.h"
 
@@ -243,6 +244,42 @@ int llmgen_paged_attention(const llmgen_step_state *st, uint16_t *out, const uin
                           static_cast<const int32_t *>(st->tile_seq), static_cast<const int32_t *>(st->tile_q0),
                           st->n_tiles, st->n_head, st->n_kv_head, st->head_dim, st->max_blocks, st->block_size,
                           st->attn_scale, st->single_rows);
+    return 0;
+}
+
+int llmgen_paged_attention_form(const llmgen_step_state *st, const llmgen_cache_form *form, uint16_t *out,
+                                const uint16_t *q, const uint16_t *k, const uint16_t *v, void *k_cache, void *v_cache,
+                                int store_kv) {
+    if (!form || (!form->kv4 && form->window == 0))
+        return llmgen_paged_attention(st, out, q, k, v, static_cast<uint16_t *>(k_cache), static_cast<uint16_t *>(v_cache),
+                                      store_kv);
+    if (!st || !out || !q || !k_cache || !v_cache || form->window < 0 || form->sinks < 0) return -1;
+    if (store_kv && (!k || !v)) return -1;
+    const int32_t *slots = static_cast<const int32_t *>(st->slots);
+    const int32_t *bt = static_cast<const int32_t *>(st->block_tables);
+    const int32_t *ctx = static_cast<const int32_t *>(st->ctx);
+    const int32_t *cu_q = static_cast<const int32_t *>(st->cu_q);
+    const int32_t *ts = static_cast<const int32_t *>(st->tile_seq), *tq = static_cast<const int32_t *>(st->tile_q0);
+    uint16_t *kc = static_cast<uint16_t *>(k_cache), *vc = static_cast<uint16_t *>(v_cache);
+    uint8_t *kc4 = static_cast<uint8_t *>(k_cache), *vc4 = static_cast<uint8_t *>(v_cache);
+    const int nq = st->n_head, nkv = st->n_kv_head, hd = st->head_dim, mb = st->max_blocks, bs = st->block_size;
+    const int longest = (int)std::min<size_t>(st->max_model_len, 0x3fffffff);
+    if (store_kv) {
+        if (form->kv4) hip_store_kv4(k, v, slots, kc4, vc4, st->n_tok, nkv, hd, bs);
+        else hip_store_kv(k, v, slots, kc, vc, st->n_tok, nkv, hd, bs);
+    }
+    if (st->decode && form->kv4)
+        hip_attn_decode_kv4(out, q, kc4, vc4, bt, ctx, st->n_seq, nq, nkv, hd, mb, bs, st->attn_scale, form->window,
+                            form->sinks, longest, form->work, form->work_bytes);
+    else if (st->decode)
+        hip_attn_decode_window(out, q, kc, vc, bt, ctx, st->n_seq, nq, nkv, hd, mb, bs, st->attn_scale, form->window,
+                               form->sinks, longest, form->work, form->work_bytes);
+    else if (form->kv4)
+        hip_attn_prefill_kv4(out, q, kc4, vc4, bt, ctx, cu_q, ts, tq, st->n_tiles, nq, nkv, hd, mb, bs, st->attn_scale,
+                             form->window, form->sinks, st->single_rows, form->work, form->work_bytes);
+    else
+        hip_attn_prefill_window(out, q, kc, vc, bt, ctx, cu_q, ts, tq, st->n_tiles, nq, nkv, hd, mb, bs, st->attn_scale,
+                                form->window, form->sinks, st->single_rows, form->work, form->work_bytes);
     return 0;
 }
 

@@ -1,0 +1,527 @@
+// kv4.hip -- the paged KV cache held in 4 bits: writing rows into it, reading them back, and split-K decode over it
+// (contracts in include/llmgen_cache.h; the causal prefill over 4-bit pages is in window.hip).
+//
+// Mathematics: a run of 32 values x shares a power of two 2^e, and value x is held as the e2m1 grid value nearest to
+// x / 2^e.  Dequantisation is exact in bf16 (two bits of mantissa and a power of two), so attention over the pages is
+// attention over bf16 rows that are read at 68 bytes each instead of 256.
+#include "cache_common.h"
+
+#include <algorithm>
+
+namespace {
+
+using namespace llmgen_cache;
+
+// ------------------------------------------------------------------------------------------------------------
+// Writing and reading back
+// ------------------------------------------------------------------------------------------------------------
+// HBM-bound copies with a conversion: 16 lanes take a row, 8 values (16 bytes of bf16, 4 bytes of codes) each, so a wave
+// moves 1 KB of bf16 in one access; the largest magnitude of a run of 32 is an integer maximum over the 4 lanes that
+// hold it (two DPP steps), and the conversion itself is the hardware's, two values an instruction.
+constexpr int ROW_LANES = 16, QUANT_THREADS = 256;
+
+// one step of a maximum over the quad
+template <int CTRL>
+__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false));
+}
+
+// where row `row` = (token, kv head) of K or V goes: byte offset of its codes, and of its scales
+__device__ __forceinline__ void row_place(int slot, int h, int nkv, int block_size, long &codes, long &scales) {
+    const int blk = slot / block_size, off = slot - blk * block_size;
+    const long base = ((long)blk * nkv + h) * head_bytes(block_size);
+    codes = base + (long)off * CODE_BYTES;
+    scales = base + (long)block_size * CODE_BYTES + (long)off * SCALE_BYTES;
+}
+
+__global__ void __launch_bounds__(QUANT_THREADS) store_kv4_kernel(const bf16_t *__restrict__ k,
+                                                                  const bf16_t *__restrict__ v,
+                                                                  const int *__restrict__ slots,
+                                                                  uint8_t *__restrict__ kc, uint8_t *__restrict__ vc,
+                                                                  long rows, int nkv, int block_size) {
+    const long idx = (long)blockIdx.x * QUANT_THREADS + threadIdx.x;
+    const long r = idx / ROW_LANES;
+    const int c = (int)(idx % ROW_LANES);
+    if (r >= 2 * rows) return;  // whole rows leave together, so the quads below are full
+    const bool is_v = r >= rows;
+    const long row = is_v ? r - rows : r;
+    const int t = (int)(row / nkv), h = (int)(row - (long)t * nkv);
+    const int slot = slots[t];
+    if (slot < 0) return;
+    const u32x4_t x = ld16((is_v ? v : k) + row * HD + c * 8);
+    uint32_t top = 0;  // magnitude bits: they order as the values do, infinities and NaN above all
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(top, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
+    top = quad_max<0xB1>(top);
+    top = quad_max<0x4E>(top);
+    // floor(log2 amax) is the exponent field for normal numbers.  Subnormal ones have an amax below 2^-126, and e would
+    // fall below -127 for any amax under 2^-125: both take the clamp.  Mantissas above 1.75 (0x60 of 7 bits) round up.
+    const int field = (int)(top >> 7);
+    int byte = field - 2 + ((top & 0x7f) > 0x60 ? 1 : 0);
+    byte = top == 0 ? 0 : min(max(byte, 0), 252);
+    const bool bad = top >= 0x7f80u;
+    if (bad) byte = 255;
+    const float s = kv4_scale(bad ? 127 : byte);
+    const uint32_t x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x0), s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x1), s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x2), s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x3), s, 3);
+    if (bad) w = 0;
+    long codes, scales;
+    row_place(slot, h, nkv, block_size, codes, scales);
+    uint8_t *pool = is_v ? vc : kc;
+    *reinterpret_cast<uint32_t *>(pool + codes + c * 4) = w;
+    if ((c & 3) == 0) pool[scales + (c >> 2)] = (uint8_t)byte;
+}
+
+__global__ void __launch_bounds__(QUANT_THREADS) load_kv4_kernel(bf16_t *__restrict__ k, bf16_t *__restrict__ v,
+                                                                 const int *__restrict__ slots,
+                                                                 const uint8_t *__restrict__ kc,
+                                                                 const uint8_t *__restrict__ vc, long rows, int nkv,
+                                                                 int block_size) {
+    const long idx = (long)blockIdx.x * QUANT_THREADS + threadIdx.x;
+    const long r = idx / ROW_LANES;
+    const int c = (int)(idx % ROW_LANES);
+    if (r >= 2 * rows) return;
+    const bool is_v = r >= rows;
+    const long row = is_v ? r - rows : r;
+    const int t = (int)(row / nkv), h = (int)(row - (long)t * nkv);
+    const int slot = slots[t];
+    if (slot < 0) return;
+    long codes, scales;
+    row_place(slot, h, nkv, block_size, codes, scales);
+    const uint8_t *pool = is_v ? vc : kc;
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(pool + codes + c * 4);
+    const float s = kv4_scale(pool[scales + (c >> 2)]);
+    *reinterpret_cast<u32x4_t *>((is_v ? v : k) + row * HD + c * 8) = kv4_to_bf16(w, s);
+}
+
+bool check_rows(const char *who, const void *k, const void *v, const void *slots, const void *kc, const void *vc, int T,
+                int nkv, int hd, int block_size) {
+    if (!k || !v || !slots || !kc || !vc) return refuse(who, "a tensor is missing");
+    if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc) & 15)
+        return refuse(who, "tensors must be 16-byte aligned");
+    if (hd != HD || nkv <= 0 || block_size <= 0) return refuse(who, "unsupported shape (head_dim must be 128)");
+    if ((long)T * nkv * 2 * ROW_LANES / QUANT_THREADS >= 0x7fffffffL) return refuse(who, "too many rows");
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// Split-K decode
+// ------------------------------------------------------------------------------------------------------------
+// One workgroup of 4 waves takes a span of one (sequence, kv head)'s visible keys, in tiles of 16 keys; a wave takes NT
+// tiles (NT * 16 keys, 8.5 KB of codes and scales at NT = 4) a round and works alone until the end.
+//   * K: lane (row l % 16, run l / 16) loads the 16 bytes that hold 32 values of one key, so a tile is one contiguous
+//     kilobyte in one access, and converts them to four A fragments of v_mfma_f32_16x16x32_bf16 in registers.  Step c of
+//     the product takes values 8c..8c+7 of every run; q is loaded in the same order, so no lane exchange is needed.
+//     (The scaled fp8 x fp4 product would take the codes as they are, with q split exactly into two fp8 parts, but its
+//     inner sums are kept to fewer bits: 9e-4 off on dot products of up to 59, where this one is exact to 2e-6.)
+//   * S^T = K Q^T puts the tile's keys in rows (4 a lane) and the group's heads in columns, so the softmax over keys is
+//     lane-local plus two lane exchanges, the running maximum and sum live in the lanes of their head, and two tiles'
+//     probabilities, rounded to bf16 (half a step, 2^-9, as the other attention kernels), are the B fragment of
+//     O^T = V^T P^T as they stand: the fragment's k-slots are assigned to keys in the order the accumulator holds them.
+//   * V: lane l loads bytes 16 l of the tile (key l / 4, run l % 4), converts them and puts the bf16 row into the wave's
+//     8 KB of LDS, from where ds_read_b64_tr_b16 reads it transposed.  Chunks of 16 bytes are swizzled by the row
+//     (chunk ^ 2 (row & 7)) so that both directions spread over the banks.
+//   * The loads of a round are issued when the registers they go to were just converted, a round ahead of their use.
+// The waves' (m, l, O) are merged through LDS; a sequence with several spans leaves them in the caller's scratch, and
+// the last workgroup of the (sequence, kv head) to finish merges them, by a counter that returns to 0.
+constexpr int NW = 4;         // waves a workgroup
+constexpr int TILE = 16;      // keys a tile
+constexpr int MAX_PARTS = 256;  // spans a sequence: their weights for 16 heads fill the 32 KB of LDS when merging
+
+struct DecodeLds {
+    __attribute__((aligned(16))) unsigned char v[NW][32 * HD * 2];
+    float m[NW][16];
+    float l[NW][16];
+    int last;
+};
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+__device__ __forceinline__ s16x4_t ds_read_tr(const bf16_t *p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)p);
+}
+
+// maximum / sum over the four lanes l % 16 of a wave's 16-lane groups
+__device__ __forceinline__ float group_max(float x) {
+    x = fmaxf(x, lane_xor(x, 16));
+    return fmaxf(x, lane_xor(x, 32));
+}
+__device__ __forceinline__ float group_sum(float x) {
+    x += lane_xor(x, 16);
+    return x + lane_xor(x, 32);
+}
+
+__device__ __forceinline__ u32x4_t ld16_stream(const void *p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(p));
+}
+
+// PAGE16: block_size % 16 == 0, a tile lies inside one page (one block-table read a tile, in scalar registers); else
+// each lane looks its own key's page up.
+template <bool PAGE16, int NT>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)))
+    attn_decode_kv4_kernel(bf16_t *__restrict__ out, const bf16_t *__restrict__ q, const uint8_t *__restrict__ kc,
+                           const uint8_t *__restrict__ vc, const int *__restrict__ block_tables,
+                           const int *__restrict__ ctx_lens, const int *__restrict__ cu_q,
+                           const int *__restrict__ tile_seq, int S, int nq, int nkv, int G, int max_blocks,
+                           int block_size, int bs_shift, float scale_log2, int window, int sinks, int span0, int nparts,
+                           float *__restrict__ part_o, float *__restrict__ part_ml, int *__restrict__ counters) {
+    __shared__ DecodeLds sm;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, rgrp = lane >> 4;
+    const int kvh = blockIdx.x % nkv;
+    const long rest = blockIdx.x / nkv;
+    const int by = (int)(rest % S), part = (int)(rest / S);
+    // a decode launch: `by` is the sequence and its row; a launch over a prefill step's tile list (cu_q): the single
+    // rows of it, from the end of the list (longest first), one span each
+    int s = by, row = by;
+    if (cu_q) {
+        s = tile_seq[S - 1 - by];
+        row = cu_q[s];
+        if (cu_q[s + 1] - row != 1) return;
+    }
+    const int ctx = (int)min((long)ctx_lens[s], (long)max_blocks * block_size);
+    if (ctx <= 0) {
+        if (part == 0)
+            for (int i = tid; i < G * HD / 2; i += 64 * NW)
+                reinterpret_cast<uint32_t *>(out + ((long)row * nq + (long)kvh * G) * HD)[i] = 0;
+        return;
+    }
+    // visible keys: [0, sinks) and [lo, ctx).  Tiles are counted over both: st tiles of sinks, then from lo's tile on.
+    const int lo = max(0, ctx - window);
+    const int lo_tile = lo / TILE;
+    const int st = min((sinks + TILE - 1) / TILE, lo_tile);
+    const int gap = (lo_tile - st) * TILE;
+    const int nt = (ctx + TILE - 1) / TILE - (lo_tile - st);
+    const int span = max(span0, ((nt + nparts - 1) / nparts + NT - 1) / NT * NT);  // tiles a workgroup
+    const int np = (nt + span - 1) / span;
+    if (part >= np) return;
+    const int t_end = min(nt, (part + 1) * span);
+
+    const long hb = head_bytes(block_size), page = hb * nkv;
+    const int *bt = block_tables + (long)s * max_blocks;
+    const uint8_t *kbase = kc + kvh * hb, *vbase = vc + kvh * hb;
+    const long scale_at = (long)block_size * CODE_BYTES;
+
+    // B operand: column col is head kvh * G + col (columns past G hold zeros and are never stored); step c holds values
+    // rgrp * 32 + 8 c .. + 8
+    bf16x8_t qf[4];
+    {
+        const bf16_t *qp = q + ((long)row * nq + (long)kvh * G + (col < G ? col : 0)) * HD + rgrp * 32;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            u32x4_t x = ld16(qp + c * 8);
+            if (col >= G) x = u32x4_t{0, 0, 0, 0};
+            qf[c] = __builtin_bit_cast(bf16x8_t, x);
+        }
+    }
+    f32x4_t o[8];  // O^T: dims db * 16 + rgrp * 4 + i of head col
+#pragma unroll
+    for (int db = 0; db < 8; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.f;
+
+    u32x4_t kreg[NT], vreg[NT];
+    uint32_t ksc[NT], vsc[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        kreg[i] = vreg[i] = u32x4_t{0, 0, 0, 0};
+        ksc[i] = vsc[i] = 0;
+    }
+    auto tile_key = [&](int vt) { return vt * TILE + (vt >= st ? gap : 0); };
+    auto seen = [&](int t) { return t < ctx && (t >= lo || t < sinks); };
+    // byte offset of key t's codes and scales in the pool; a key that is not visible is replaced by one that is
+    auto place = [&](int t, long &codes, long &scales) {
+        t = min(t, ctx - 1);
+        if (t >= sinks && t < lo) t = lo;
+        const int blk = bs_shift >= 0 ? t >> bs_shift : t / block_size;
+        const int off = t - blk * block_size;
+        const long base = (long)bt[blk] * page;
+        codes = base + (long)off * CODE_BYTES;
+        scales = base + scale_at + (long)off * SCALE_BYTES;
+    };
+    auto load = [&](const uint8_t *pool, int vt, int r, int run, u32x4_t &x, uint32_t &sc) {
+        if (vt >= t_end) return;  // uniform across the wave
+        const int t0 = tile_key(vt);
+        if (PAGE16) {
+            const int blk = bs_shift >= 0 ? t0 >> bs_shift : t0 / block_size;
+            const int off = t0 - blk * block_size;
+            const uint8_t *p = pool + (long)bt[blk] * page + (long)off * CODE_BYTES;
+            const uint8_t *ps = pool + (long)bt[blk] * page + scale_at + off * SCALE_BYTES;
+            x = ld16_stream(p + r * CODE_BYTES + run * 16);
+            sc = ps[r * SCALE_BYTES + run];
+        } else {
+            long codes, scales;
+            place(t0 + r, codes, scales);
+            x = ld16_stream(pool + codes + run * 16);
+            sc = pool[scales + run];
+        }
+    };
+    auto load_k = [&](int vt0) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) load(kbase, vt0 + i, col, rgrp, kreg[i], ksc[i]);
+    };
+    auto load_v = [&](int vt0) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) load(vbase, vt0 + i, lane >> 2, lane & 3, vreg[i], vsc[i]);
+    };
+
+    bf16_t *vl = reinterpret_cast<bf16_t *>(sm.v[wave]);
+    int vt0 = part * span + wave * NT;
+    if (vt0 < t_end) {
+        load_k(vt0);
+        load_v(vt0);
+    }
+    for (; vt0 < t_end; vt0 += NW * NT) {
+        const int next = vt0 + NW * NT;
+        // ---- scores ----
+        f32x4_t sc[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const float s2 = kv4_scale(ksc[i]);
+            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kv4_to_bf16(kreg[i][c], s2)),
+                                                              qf[c], acc, 0, 0, 0);
+            sc[i] = acc;
+        }
+        if (next < t_end) load_k(next);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int t0 = tile_key(vt0 + i);
+            // whole tiles are visible except at the ends of the sinks, the window and the sequence (uniform)
+            const bool whole = vt0 + i < t_end && t0 + TILE <= ctx && (t0 >= lo || t0 + TILE <= sinks);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sc[i][j] *= scale_log2;
+                if (!whole && !(vt0 + i < t_end && seen(t0 + rgrp * 4 + j))) sc[i][j] = -INFINITY;
+                mx = fmaxf(mx, sc[i][j]);
+            }
+            if (!whole && !seen(t0 + (lane >> 2))) vsc[i] = 0;  // finite values behind a probability of 0
+        }
+        // ---- online softmax of head col ----
+        mx = group_max(mx);
+        const float m_new = fmaxf(m_run, mx);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        if (__any(m_new > m_run)) {
+            const float corr = fast_exp2(m_run - m_use);
+            l_run *= corr;
+#pragma unroll
+            for (int db = 0; db < 8; ++db)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[db][j] *= corr;
+        }
+        m_run = m_new;
+        u32x2_t p[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            float e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                e[j] = fast_exp2(sc[i][j] - m_use);
+                l_run += e[j];
+            }
+            p[i] = u32x2_t{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
+        }
+        // ---- O^T += V^T P^T, two tiles (32 keys) a step ----
+#pragma unroll
+        for (int h = 0; h < NT / 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float s2 = kv4_scale(vsc[2 * h + i]);
+                const int r = i * 16 + (lane >> 2);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int chunk = ((lane & 3) * 4 + c) ^ ((r & 7) << 1);
+                    *reinterpret_cast<u32x4_t *>(vl + r * HD + chunk * 8) = kv4_to_bf16(vreg[2 * h + i][c], s2);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            const u32x4_t pw = {p[2 * h][0], p[2 * h][1], p[2 * h + 1][0], p[2 * h + 1][1]};
+            const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, pw);
+            const int r = rgrp * 4 + (col >> 2);  // this lane's row of a transposed read, in either tile
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+                const int chunk = (db * 2 + ((col & 3) >> 1)) ^ ((r & 7) << 1);
+                const bf16_t *src = vl + r * HD + chunk * 8 + (col & 1) * 4;
+                const s16x4_t a0 = ds_read_tr(src), a1 = ds_read_tr(src + 16 * HD);
+                o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7)), pb, o[db], 0, 0,
+                    0);
+            }
+            // the rows are overwritten next: keep every lane's reads ahead of those writes
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        }
+        if (next < t_end) load_v(next);
+    }
+
+    // ---- merge the waves ----
+    l_run = group_sum(l_run);
+    if (rgrp == 0) {
+        sm.m[wave][col] = m_run;
+        sm.l[wave][col] = l_run;
+    }
+    if (col < G) {
+        float *ow = reinterpret_cast<float *>(sm.v[wave]) + col * HD;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4_t *>(ow + db * 16 + rgrp * 4) = o[db];
+    }
+    __syncthreads();
+    for (int idx = tid; idx < G * HD; idx += 64 * NW) {
+        const int g = idx / HD, d = idx % HD;
+        float M = sm.m[0][g];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) M = fmaxf(M, sm.m[w][g]);
+        const float Mu = M == -INFINITY ? 0.f : M;
+        float acc = 0.f, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float e = fast_exp2(sm.m[w][g] - Mu);
+            acc += e * reinterpret_cast<const float *>(sm.v[w])[idx];
+            L += e * sm.l[w][g];
+        }
+        const long h = (long)kvh * G + g;
+        if (np == 1) {
+            out[((long)row * nq + h) * HD + d] = __builtin_bit_cast(bf16_t, (__bf16)(acc / L));
+        } else {  // device-coherent stores: another workgroup reads them
+            const long slot = ((long)s * nq + h) * nparts + part;
+            __hip_atomic_store(part_o + slot * HD + d, acc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (d == 0) {
+                __hip_atomic_store(part_ml + slot * 2, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(part_ml + slot * 2 + 1, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+    }
+    if (np == 1) return;
+
+    // ---- merge the spans: every thread's stores are complete before the barrier, then one counter increment a
+    //      workgroup elects the last, which reads the partials with device-coherent loads, in span order ----
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    int *cnt = counters + (long)s * nkv + kvh;
+    if (tid == 0) sm.last = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == np - 1;
+    __syncthreads();
+    if (!sm.last) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    auto ld = [](const float *x) { return __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    float *ml = reinterpret_cast<float *>(sm.v);  // [head][span][m, l]
+    const long slot0 = ((long)s * nq + (long)kvh * G) * nparts;
+    for (int i = tid; i < G * np; i += 64 * NW) {
+        const int g = i / np, p = i - g * np;
+        const float *src = part_ml + (slot0 + (long)g * nparts + p) * 2;
+        ml[2 * i] = ld(src);
+        ml[2 * i + 1] = ld(src + 1);
+    }
+    __syncthreads();
+    constexpr int MB = 16;  // partials a thread has in flight
+    for (int idx = tid; idx < G * HD; idx += 64 * NW) {
+        const int g = idx / HD, d = idx % HD;
+        const float *mlg = ml + 2 * g * np;
+        const float *po = part_o + (slot0 + (long)g * nparts) * HD + d;
+        float M = -INFINITY, num = 0.f, den = 0.f;
+        for (int p = 0; p < np; ++p) M = fmaxf(M, mlg[2 * p]);
+        const float Mu = M == -INFINITY ? 0.f : M;
+        for (int p0 = 0; p0 < np; p0 += MB) {
+            float ov[MB];
+#pragma unroll
+            for (int j = 0; j < MB; ++j) ov[j] = p0 + j < np ? ld(po + (long)(p0 + j) * HD) : 0.f;
+#pragma unroll
+            for (int j = 0; j < MB; ++j)
+                if (p0 + j < np) {
+                    const float w = fast_exp2(mlg[2 * (p0 + j)] - Mu);
+                    num += w * ov[j];
+                    den += w * mlg[2 * (p0 + j) + 1];
+                }
+        }
+        out[((long)row * nq + (long)kvh * G + g) * HD + d] = __builtin_bit_cast(bf16_t, (__bf16)(num / den));
+    }
+    if (tid == 0) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+struct DecodeShape {
+    int S, nq, nkv, G, max_blocks, block_size;
+    float sl2;
+    int window, sinks;
+};
+
+void launch_decode(bf16_t *out, const bf16_t *q, const uint8_t *kc, const uint8_t *vc, const int *bt, const int *ctx,
+                   const int *cu_q, const int *tile_seq, const DecodeShape &d, int span, int nparts, const Work &w) {
+    constexpr int NT = 4;
+    const int bs_shift = (d.block_size & (d.block_size - 1)) == 0 ? __builtin_ctz(d.block_size) : -1;
+    const long rows = (long)d.S * d.nq * nparts;
+    float *part_o = nparts > 1 ? w.part : nullptr, *part_ml = nparts > 1 ? w.part + rows * HD : nullptr;
+    auto kern = d.block_size % TILE == 0 ? attn_decode_kv4_kernel<true, NT> : attn_decode_kv4_kernel<false, NT>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)d.nkv * d.S * nparts)), dim3(64 * NW), 0, g_llmgen_stream, out, q, kc,
+                       vc, bt, ctx, cu_q, tile_seq, d.S, d.nq, d.nkv, d.G, d.max_blocks, d.block_size, bs_shift, d.sl2,
+                       d.window, d.sinks, span, nparts, part_o, part_ml, w.counters);
+}
+
+}  // namespace
+
+extern "C" size_t hip_kv4_block_bytes(int nkv, int hd, int block_size) {
+    if (hd != HD || nkv <= 0 || block_size <= 0) return 0;
+    return (size_t)nkv * head_bytes(block_size);
+}
+
+extern "C" void hip_store_kv4(const bf16_t *k, const bf16_t *v, const int *slot_mapping, uint8_t *k_cache,
+                              uint8_t *v_cache, int T, int nkv, int hd, int block_size) {
+    if (T <= 0 || !check_rows("store_kv4", k, v, slot_mapping, k_cache, v_cache, T, nkv, hd, block_size)) return;
+    const long rows = (long)T * nkv;
+    const long blocks = (2 * rows * ROW_LANES + QUANT_THREADS - 1) / QUANT_THREADS;
+    hipLaunchKernelGGL(store_kv4_kernel, dim3((unsigned)blocks), dim3(QUANT_THREADS), 0, g_llmgen_stream, k, v,
+                       slot_mapping, k_cache, v_cache, rows, nkv, block_size);
+}
+
+extern "C" void hip_load_kv4(bf16_t *k, bf16_t *v, const int *slot_mapping, const uint8_t *k_cache,
+                             const uint8_t *v_cache, int T, int nkv, int hd, int block_size) {
+    if (T <= 0 || !check_rows("load_kv4", k, v, slot_mapping, k_cache, v_cache, T, nkv, hd, block_size)) return;
+    const long rows = (long)T * nkv;
+    const long blocks = (2 * rows * ROW_LANES + QUANT_THREADS - 1) / QUANT_THREADS;
+    hipLaunchKernelGGL(load_kv4_kernel, dim3((unsigned)blocks), dim3(QUANT_THREADS), 0, g_llmgen_stream, k, v,
+                       slot_mapping, k_cache, v_cache, rows, nkv, block_size);
+}
+
+extern "C" void hip_attn_decode_kv4(bf16_t *out, const bf16_t *q, const uint8_t *k_cache, const uint8_t *v_cache,
+                                    const int *block_tables, const int *ctx_lens, int S, int nq, int nkv, int hd,
+                                    int max_blocks, int block_size, float scale, int window, int sinks, int max_ctx,
+                                    void *work, size_t work_bytes) {
+    const char *who = "attn_decode_kv4";
+    if (S <= 0 || !check_attention(who, out, q, k_cache, v_cache, block_tables, ctx_lens, nq, nkv, hd, max_blocks,
+                                   block_size, scale, window, sinks, work))
+        return;
+    DecodeShape d{S, nq, nkv, nq / nkv, max_blocks, block_size, scale * LLMGEN_LOG2E,
+                  window ? std::min(window, NO_WINDOW) : NO_WINDOW, std::min(sinks, NO_WINDOW)};
+    const Work w = split_work(work, work_bytes);
+    // Tiles of the longest expected sequence, and spans so that the launch has about four workgroups a CU; a span is at
+    // least one round of the four waves.
+    long keys = std::max(1, std::min(max_ctx, max_blocks * block_size));
+    keys = std::min(keys, (long)d.window + d.sinks + 2 * TILE);
+    const long tiles = (keys + TILE - 1) / TILE;
+    constexpr int ROUND = NW * 4;
+    long parts = std::min<long>({(4L * llmgen_num_cus() + (long)S * nkv - 1) / ((long)S * nkv),
+                                 (tiles + ROUND - 1) / ROUND, MAX_PARTS, w.floats / ((long)S * nq * (HD + 2))});
+    if (parts < 1 || (long)S * nkv > WORK_COUNTERS) parts = 1;
+    const long span = ((tiles + parts - 1) / parts + 3) / 4 * 4;
+    if ((long)nkv * S * parts > 0x7fffffffL) {
+        refuse(who, "too many sequences");
+        return;
+    }
+    launch_decode(out, q, k_cache, v_cache, block_tables, ctx_lens, nullptr, nullptr, d, (int)span, (int)parts, w);
+}
+
+// The single rows of a prefill step over 4-bit pages: one workgroup a (row, kv head).
+void llmgen_kv4_rows_of_prefill(bf16_t *out, const bf16_t *q, const uint8_t *k_cache, const uint8_t *v_cache,
+                                const int *block_tables, const int *ctx_lens, const int *cu_q, const int *tile_seq,
+                                int n_tiles, int nq, int nkv, int max_blocks, int block_size, float scale_log2, int window,
+                                int sinks) {
+    DecodeShape d{n_tiles, nq, nkv, nq / nkv, max_blocks, block_size, scale_log2, window, sinks};
+    launch_decode(out, q, k_cache, v_cache, block_tables, ctx_lens, cu_q, tile_seq, d, 1 << 26, 1, Work{});
+}

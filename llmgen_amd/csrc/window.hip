@@ -1,0 +1,271 @@
+// window.hip -- attention with a sliding window and sinks over bf16 pages, and causal prefill over 4-bit pages with or
+// without them (gfx950; contracts in include/llmgen_cache.h).
+//
+// A row at position p sees keys k <= p with k > p - window or k < sinks; without a window that is plain causal
+// attention.  What bounds these kernels is what bounds attention over the whole context -- HBM for one query row a
+// sequence, the matrix cores for many -- so they are built from the same workgroups, and the work they save is the keys
+// they do not walk: a decode row reads window + sinks keys whatever its context, and a query tile of 64 rows walks the
+// 64-key tiles of the sinks and of its own window, of which only those cut by an end of either, or by the diagonal, pay
+// for masks.
+//   * decode over bf16 pages: the split-K workgroup of decode_kernel.h, walking the visible keys only;
+//   * prefill: the workgroup of window_kernel.h.  A unit is a query tile x KV head x group of NW / 2 heads; with few
+//     units each one's key tiles are split over up to 8 workgroups, whose partial (m, l, O) the last to finish merges in
+//     order out of the caller's scratch;
+//   * 4-bit pages: a tile's codes are loaded a tile ahead into registers (one 16-byte run of 32 codes of K and one of V
+//     a thread) and converted to bf16 on the way into LDS, so the products and the softmax are the same code;
+//   * single rows of a prefill step are streamed by a decode launch before it.
+#include "cache_common.h"
+#include "decode_kernel.h"
+#include "hip_common.h"
+#include "window_kernel.h"
+
+#include <algorithm>
+
+namespace {
+
+using llmgen_cache::check_attention;
+using llmgen_cache::NO_WINDOW;
+using llmgen_cache::refuse;
+using llmgen_cache::split_work;
+using llmgen_cache::Work;
+using llmgen_cache::WORK_COUNTERS;
+
+// ------------------------------------------------------------------------------------------------------------
+// Decode over bf16 pages
+// ------------------------------------------------------------------------------------------------------------
+struct RowArgs {
+    bf16_t *out;
+    const bf16_t *q, *kc, *vc;
+    const int *bt, *ctx, *cu_q, *tile_seq;
+    int S, nq, nkv, max_blocks, block_size, bs_shift;
+    float sl2;
+    int window, sinks, span, nparts;
+    float *part_o, *part_ml;
+    int *counters;
+};
+
+template <int G, int NT, bool POW2, int W>
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(G == 4 && W == 8 ? 2 : 3)))
+    attn_decode_window_kernel(const RowArgs a) {
+    using namespace llmgen_decode;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[sizeof(DecodeLds<G, NT, W>)];
+    const int kvh = blockIdx.x % a.nkv;
+    const long rest = blockIdx.x / a.nkv;
+    decode_split_body<G, NT, POW2, false, W, true>(
+        a.out, a.part_o, a.part_ml, a.q, a.kc, a.vc, a.bt, a.ctx, a.nq, a.nkv, a.max_blocks, a.block_size, a.bs_shift,
+        a.sl2, a.span, a.nparts, a.nparts, a.counters, a.cu_q, a.tile_seq, nullptr, nullptr, nullptr, nullptr, nullptr,
+        kvh, (int)(rest % a.S), (int)(rest / a.S), a.S, lds, a.window, a.sinks);
+}
+
+template <int G, int NT, int W>
+void launch_rows(const RowArgs &a) {
+    auto kern = a.bs_shift >= 0 ? attn_decode_window_kernel<G, NT, true, W> : attn_decode_window_kernel<G, NT, false, W>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.nkv * a.S * a.nparts)), dim3(64 * W), 0, g_llmgen_stream, a);
+}
+
+void launch_rows_g(const RowArgs &a, int waves) {
+    switch (a.nq / a.nkv) {
+        case 1: waves == 8 ? launch_rows<1, 2, 8>(a) : launch_rows<1, 2, 4>(a); break;
+        case 2: waves == 8 ? launch_rows<2, 2, 8>(a) : launch_rows<2, 2, 4>(a); break;
+        case 4: waves == 8 ? launch_rows<4, 2, 8>(a) : launch_rows<4, 2, 4>(a); break;
+        case 8: launch_rows<8, 2, 4>(a); break;
+        default: launch_rows<16, 1, 4>(a); break;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// Prefill
+// ------------------------------------------------------------------------------------------------------------
+constexpr int PIECES_MAX = 8, PIECE_MIN_TILES = 4;
+
+template <int NW, int MODE>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
+    attn_prefill_window_kernel(const llmgen_window::WindowArgs a, int n_units, int P, float *__restrict__ part,
+                               int *__restrict__ counters) {
+    using namespace llmgen_window;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[sizeof(WindowLds<NW>)];
+    if constexpr (NW <= 4) {
+        if (P > 1) {
+            __shared__ int s_last;
+            const int unit = (int)(blockIdx.x % n_units), piece = (int)(blockIdx.x / n_units);
+            const int tile = a.n_tiles - 1 - unit / (a.nkv * a.head_groups);
+            const int s = a.tile_seq[tile], q0 = a.tile_q0[tile], q_len = a.cu_q[s + 1] - a.cu_q[s];
+            const int ctx = (int)min((long)a.ctx_lens[s], (long)a.max_blocks * a.block_size);
+            const int n = (q_len > 1 || a.single) && ctx >= q_len
+                              ? key_tiles(ctx - q_len + q0, ctx - q_len + min(q0 + BQ, q_len), a.window, a.sinks).n
+                              : 0;
+            const int pe = n < 2 ? 1 : min(P, (n + PIECE_MIN_TILES - 1) / PIECE_MIN_TILES);
+            if (piece >= pe) return;
+            if (pe > 1) {
+                constexpr int PSTRIDE = NW * PART_WAVE_FLOATS;
+                float *base = part + (long)unit * P * PSTRIDE;
+                window_body<NW, MODE>(a, unit, lds, (int)((long)piece * n / pe), (int)((long)(piece + 1) * n / pe),
+                                      base + (long)piece * PSTRIDE);
+                // publish (device-coherent stores, complete before the barrier), then draw a ticket: the last merges
+                __builtin_amdgcn_s_waitcnt(0);
+                __syncthreads();
+                if (threadIdx.x == 0)
+                    s_last = __hip_atomic_fetch_add(counters + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                             pe - 1;
+                __syncthreads();
+                if (!s_last) return;
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+                prefill_merge_store_n<PIECES_MAX, NW>(a.out, a.cu_q, a.tile_seq, a.tile_q0, a.n_tiles, a.nq, a.nkv, a.G,
+                                                      a.head_groups, unit, base, pe);
+                if (threadIdx.x == 0)
+                    __hip_atomic_store(counters + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                return;
+            }
+            window_body<NW, MODE>(a, unit, lds, 0, -1, nullptr);
+            return;
+        }
+    }
+    window_body<NW, MODE>(a, blockIdx.x, lds, 0, -1, nullptr);
+}
+
+template <int NW>
+void launch_prefill(int mode, const llmgen_window::WindowArgs &a, long units, int P, const Work &w) {
+    auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, dim3((unsigned)(units * P)), dim3(64 * NW), 0, g_llmgen_stream, a, (int)units, P, w.part,
+                           w.counters);
+    };
+    using namespace llmgen_window;
+    if (mode == KV4) go(attn_prefill_window_kernel<NW, KV4>);
+    else if (mode == DMA_BLOCK) go(attn_prefill_window_kernel<NW, DMA_BLOCK>);
+    else if (mode == DMA_ROW4) go(attn_prefill_window_kernel<NW, DMA_ROW4>);
+    else go(attn_prefill_window_kernel<NW, DMA_FLAT>);
+}
+
+void prefill(const char *who, bool kv4, bf16_t *out, const bf16_t *q, const void *kc, const void *vc, const int *bt,
+             const int *ctx, const int *cu_q, const int *tile_seq, const int *tile_q0, int n_tiles, int nq, int nkv,
+             int hd, int max_blocks, int block_size, float scale, int window, int sinks, int single_rows, void *work,
+             size_t work_bytes) {
+    if (n_tiles <= 0 || !check_attention(who, out, q, kc, vc, bt, ctx, nq, nkv, hd, max_blocks, block_size, scale, window,
+                                         sinks, work))
+        return;
+    if (!cu_q || !tile_seq || !tile_q0) {
+        refuse(who, "a tensor is missing");
+        return;
+    }
+    const int G = nq / nkv;
+    const int bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
+    const float sl2 = scale * LLMGEN_LOG2E;
+    window = window ? std::min(window, NO_WINDOW) : NO_WINDOW;
+    sinks = std::min(sinks, NO_WINDOW);
+    using namespace llmgen_window;
+    const int mode = kv4 ? KV4
+                   : bs_shift >= 0 && block_size % BK == 0 ? (int)DMA_BLOCK
+                   : block_size % 4 == 0                   ? (int)DMA_ROW4
+                                                           : (int)DMA_FLAT;
+    // one head a 2-wave workgroup at G = 1, two a 4-wave one, four an 8-wave one
+    const Work w = split_work(work, work_bytes);
+    const int rows = std::max(0, std::min(single_rows, n_tiles));  // tiles that leave at once
+    int nw = G == 1 ? 2 : 4;
+    long units = (long)n_tiles * nkv * (G / (nw / 2)), busy = (long)(n_tiles - rows) * nkv * (G / (nw / 2));
+    const long slots = (long)llmgen_num_cus() * (8 / nw);  // workgroups the chip holds at once
+    long P = 1;
+    if (busy > 0 && busy * 2 <= slots && units <= WORK_COUNTERS)
+        P = std::min<long>({PIECES_MAX, slots / busy, w.floats / (units * nw * PART_WAVE_FLOATS)});
+    if (P < 1) P = 1;
+    if (P == 1 && G >= 4) {
+        nw = 8;
+        units = (long)n_tiles * nkv * (G / 4);
+    }
+    if (units * P > 0x7fffffffL || (long)n_tiles * nkv > 0x7fffffffL) {
+        refuse(who, "too many tiles");
+        return;
+    }
+    if (single_rows != 0) {
+        if (kv4) {
+            llmgen_kv4_rows_of_prefill(out, q, static_cast<const uint8_t *>(kc), static_cast<const uint8_t *>(vc), bt, ctx,
+                                       cu_q, tile_seq, n_tiles, nq, nkv, max_blocks, block_size, sl2, window, sinks);
+        } else {
+            launch_rows_g(RowArgs{out, q, static_cast<const bf16_t *>(kc), static_cast<const bf16_t *>(vc), bt, ctx, cu_q,
+                                  tile_seq, n_tiles, nq, nkv, max_blocks, block_size, bs_shift, sl2, window, sinks, 64, 1,
+                                  nullptr, nullptr, nullptr},
+                          4);
+        }
+    }
+    const WindowArgs a{out, q, kc, vc, bt, ctx, cu_q, tile_seq, tile_q0, n_tiles, nq, nkv, G, G / (nw / 2), max_blocks,
+                       block_size, bs_shift, sl2, window, sinks, single_rows == 0};
+    if (nw == 2) launch_prefill<2>(mode, a, units, (int)P, w);
+    else if (nw == 4) launch_prefill<4>(mode, a, units, (int)P, w);
+    else launch_prefill<8>(mode, a, units, 1, w);
+}
+
+__global__ void __launch_bounds__(256) clear_counters_kernel(int *counters, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) counters[i] = 0;
+}
+
+}  // namespace
+
+extern "C" size_t hip_attn_work_bytes(void) {
+    // counters, and room for 512 partial results of 4-wave prefill workgroups (or 66,000 of decode rows)
+    return llmgen_cache::WORK_HEAD + (size_t)512 * llmgen_prefill::PART_FLOATS * sizeof(float);
+}
+
+extern "C" void hip_attn_work_init(void *work, size_t work_bytes) {
+    if (!work || ((uintptr_t)work & 15)) {
+        refuse("attn_work_init", "the scratch must be 16-byte aligned device memory");
+        return;
+    }
+    const int n = (int)std::min<size_t>(work_bytes / sizeof(int), WORK_COUNTERS);
+    if (n <= 0) return;
+    hipLaunchKernelGGL(clear_counters_kernel, dim3((n + 255) / 256), dim3(256), 0, g_llmgen_stream,
+                       static_cast<int *>(work), n);
+}
+
+extern "C" void hip_attn_decode_window(bf16_t *out, const bf16_t *q, const bf16_t *k_cache, const bf16_t *v_cache,
+                                       const int *block_tables, const int *ctx_lens, int S, int nq, int nkv, int hd,
+                                       int max_blocks, int block_size, float scale, int window, int sinks, int max_ctx,
+                                       void *work, size_t work_bytes) {
+    const char *who = "attn_decode_window";
+    if (S <= 0 || !check_attention(who, out, q, k_cache, v_cache, block_tables, ctx_lens, nq, nkv, hd, max_blocks,
+                                   block_size, scale, window, sinks, work))
+        return;
+    const int G = nq / nkv;
+    const Work w = split_work(work, work_bytes);
+    window = window ? std::min(window, NO_WINDOW) : NO_WINDOW;
+    sinks = std::min(sinks, NO_WINDOW);
+    // As the decode launch over whole contexts: 8-wave workgroups where the (sequence, KV head) pairs alone nearly fill
+    // the chip, and spans of at least one round of a workgroup's waves, about 8 waves a CU in all.
+    const long pairs = (long)S * nkv;
+    const int waves = G <= 4 && pairs * 2 >= llmgen_num_cus() ? 8 : 4;
+    const int wtok = G >= 16 ? 16 : 32, round = waves * wtok;
+    long keys = std::max(1, std::min(max_ctx, max_blocks * block_size));
+    keys = std::min(keys, (long)window + sinks + wtok + 4);
+    const long target = 2L * llmgen_num_cus() * 4 / waves;
+    long parts = std::min<long>({(target + pairs - 1) / pairs, (keys + round - 1) / round, 256,
+                                 w.floats / ((long)S * nq * (llmgen_decode::HD + 2))});
+    if (parts < 1 || pairs > WORK_COUNTERS) parts = 1;
+    if (pairs * parts > 0x7fffffffL) {
+        refuse(who, "too many sequences");
+        return;
+    }
+    const long span = ((keys + parts - 1) / parts + wtok - 1) / wtok * wtok;
+    const long rows = (long)S * nq * parts;
+    launch_rows_g(RowArgs{out, q, k_cache, v_cache, block_tables, ctx_lens, nullptr, nullptr, S, nq, nkv, max_blocks,
+                          block_size, (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1,
+                          scale * LLMGEN_LOG2E, window, sinks, (int)span, (int)parts, parts > 1 ? w.part : nullptr,
+                          parts > 1 ? w.part + rows * llmgen_decode::HD : nullptr, w.counters},
+                  waves);
+}
+
+extern "C" void hip_attn_prefill_window(bf16_t *out, const bf16_t *q, const bf16_t *k_cache, const bf16_t *v_cache,
+                                        const int *block_tables, const int *ctx_lens, const int *cu_q,
+                                        const int *tile_seq, const int *tile_q0, int n_tiles, int nq, int nkv, int hd,
+                                        int max_blocks, int block_size, float scale, int window, int sinks,
+                                        int single_rows, void *work, size_t work_bytes) {
+    prefill("attn_prefill_window", false, out, q, k_cache, v_cache, block_tables, ctx_lens, cu_q, tile_seq, tile_q0,
+            n_tiles, nq, nkv, hd, max_blocks, block_size, scale, window, sinks, single_rows, work, work_bytes);
+}
+
+extern "C" void hip_attn_prefill_kv4(bf16_t *out, const bf16_t *q, const uint8_t *k_cache, const uint8_t *v_cache,
+                                     const int *block_tables, const int *ctx_lens, const int *cu_q, const int *tile_seq,
+                                     const int *tile_q0, int n_tiles, int nq, int nkv, int hd, int max_blocks,
+                                     int block_size, float scale, int window, int sinks, int single_rows, void *work,
+                                     size_t work_bytes) {
+    prefill("attn_prefill_kv4", true, out, q, k_cache, v_cache, block_tables, ctx_lens, cu_q, tile_seq, tile_q0, n_tiles,
+            nq, nkv, hd, max_blocks, block_size, scale, window, sinks, single_rows, work, work_bytes);
+}

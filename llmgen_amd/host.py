@@ -9,7 +9,9 @@ slice is implemented in C++ inside libllmgen_attn.so; this module exposes it to 
   ``PagedAttentionImpl.execute`` (executor.zig:864-895, attention_v1.zig:60-120);
 * :func:`plan_passes`, :func:`decode_buckets`, :func:`workspace` -- ``execute``/``flushPass``, ``captureGraphs``
   bucket sizes and ``Workspace.of`` (executor.zig:986-1043, 609-632, 92-102);
-* :class:`Graphs` -- decode graph buckets (captureGraphs + forward's replay path).
+* :class:`Graphs` -- decode graph buckets (captureGraphs + forward's replay path);
+* :class:`CacheForm`, :func:`paged_attention_form` -- the attention of a layer whose pages are held in 4 bits or that
+  keeps a sliding window; :class:`Blocks` -- the block manager, with pages that sequences share.
 """
 from __future__ import annotations
 
@@ -54,6 +56,13 @@ class StepState(ctypes.Structure):
                 + [("single_rows", _i32)])
 
 
+class CacheForm(ctypes.Structure):
+    """llmgen_cache_form: 4-bit pages, a sliding window and sinks, and the scratch of their launches."""
+    _fields_ = [("kv4", _i32), ("window", _i32), ("sinks", _i32), ("work", _P), ("work_bytes", _sz)]
+
+
+_i32p = ctypes.POINTER(_i32)
+
 HOST_SIGNATURES = {
     "llmgen_layout_init": (Layout, [_sz, _sz, _sz, _sz]),
     "llmgen_entry_emits": (ctypes.c_int, [ctypes.POINTER(Seq), ctypes.POINTER(Entry)]),
@@ -66,6 +75,18 @@ HOST_SIGNATURES = {
     "llmgen_bind_step": (None, [ctypes.POINTER(StepState), _P, Layout] + [ctypes.c_int] * 10
                          + [_sz, _P, _P, _P, ctypes.c_int]),
     "llmgen_paged_attention": (ctypes.c_int, [ctypes.POINTER(StepState), _P, _P, _P, _P, _P, _P, ctypes.c_int]),
+    "llmgen_paged_attention_form": (ctypes.c_int, [ctypes.POINTER(StepState), ctypes.POINTER(CacheForm), _P, _P, _P, _P,
+                                                   _P, _P, ctypes.c_int]),
+    "llmgen_blocks_create": (_P, [ctypes.c_int]),
+    "llmgen_blocks_destroy": (None, [_P]),
+    "llmgen_blocks_free_count": (ctypes.c_int, [_P]),
+    "llmgen_blocks_ref": (ctypes.c_int, [_P, ctypes.c_int]),
+    "llmgen_blocks_alloc": (ctypes.c_int, [_P, ctypes.c_int, _i32p]),
+    "llmgen_blocks_fork": (ctypes.c_int, [_P, _i32p, ctypes.c_int]),
+    "llmgen_blocks_free": (ctypes.c_int, [_P, _i32p, ctypes.c_int]),
+    "llmgen_blocks_writable": (ctypes.c_int, [_P, _i32p, ctypes.c_int, _i32p, _i32p]),
+    "llmgen_blocks_compact": (ctypes.c_int, [_P, _i32p, _i32p, ctypes.c_int]),
+    "llmgen_blocks_remap": (ctypes.c_int, [_i32p, ctypes.c_int, _i32p, _i32p, ctypes.c_int]),
     "llmgen_part_size": (ctypes.c_int, [ctypes.c_int]),
     "llmgen_max_parts": (ctypes.c_int, [ctypes.c_int, _sz]),
     "llmgen_workspace": (None, [ctypes.c_int, ctypes.c_int, ctypes.c_int, _sz, _sz, ctypes.c_int, ctypes.c_int,
@@ -201,6 +222,93 @@ def paged_attention(st: StepState, out, q, k, v, k_cache, v_cache, store_kv: boo
                                     int(store_kv))
     if rc != 0:
         raise ValueError(f"llmgen_paged_attention rejected its arguments (rc={rc})")
+
+
+def paged_attention_form(st: StepState, form: CacheForm, out, q, k, v, k_cache, v_cache, store_kv: bool = True) -> None:
+    """:func:`paged_attention` for a layer of another form of the cache; pools of 4-bit pages are uint8 tensors."""
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    rc = L().llmgen_paged_attention_form(ctypes.byref(st), ctypes.byref(form), p(out), p(q), p(k), p(v), p(k_cache),
+                                         p(v_cache), int(store_kv))
+    if rc != 0:
+        raise ValueError(f"llmgen_paged_attention_form rejected its arguments (rc={rc})")
+
+
+class OutOfBlocks(RuntimeError):
+    """No page is free."""
+
+
+class Blocks:
+    """The block manager (C++: llmgen_blocks_*): pages with reference counts.  Tables are lists of page ids; an entry
+    below 0 is a page the sequence has given back."""
+
+    def __init__(self, num_blocks: int):
+        self.num_blocks = num_blocks
+        self.h = L().llmgen_blocks_create(num_blocks)
+        if not self.h:
+            raise ValueError(f"a block manager needs at least one page, got {num_blocks}")
+
+    @staticmethod
+    def _array(table):
+        return (_i32 * max(len(table), 1))(*table)
+
+    @property
+    def free_count(self) -> int:
+        return L().llmgen_blocks_free_count(self.h)
+
+    def ref(self, block: int) -> int:
+        return L().llmgen_blocks_ref(self.h, block)
+
+    def alloc(self, n: int) -> List[int]:
+        if n < 0:
+            raise ValueError("a negative number of pages")
+        out = (_i32 * max(n, 1))()
+        if L().llmgen_blocks_alloc(self.h, n, out) != 0:
+            raise OutOfBlocks(f"{n} pages asked for, {self.free_count} free")
+        return list(out[:n])
+
+    def fork(self, table) -> List[int]:
+        """A second sequence over the same pages; returns its table."""
+        if L().llmgen_blocks_fork(self.h, self._array(table), len(table)) != 0:
+            raise ValueError("a table with pages that no sequence holds cannot be forked")
+        return list(table)
+
+    def free(self, table) -> None:
+        if L().llmgen_blocks_free(self.h, self._array(table), len(table)) != 0:
+            raise ValueError("pages given back that no sequence holds")
+
+    def writable(self, table: List[int], idx: int):
+        """Before a write into ``table[idx]``: None, or the (source, destination) of the copy to make; ``table`` then
+        holds the new page."""
+        if not 0 <= idx < len(table) or self.ref(table[idx]) <= 0:
+            raise ValueError(f"entry {idx} is not a page that a sequence holds")
+        a, src, dst = self._array(table), _i32(), _i32()
+        rc = L().llmgen_blocks_writable(self.h, a, idx, ctypes.byref(src), ctypes.byref(dst))
+        if rc < 0:
+            raise OutOfBlocks("no page is free for the copy")
+        if rc == 0:
+            return None
+        table[idx] = a[idx]
+        return src.value, dst.value
+
+    def compact(self, tables):
+        """Moves the pages in use to the lowest ids: rewrites every table in place and returns (sources, destinations),
+        int32 arrays, of the copies to make."""
+        cap = self.num_blocks
+        src, dst = (_i32 * cap)(), (_i32 * cap)()
+        n = L().llmgen_blocks_compact(self.h, src, dst, cap)
+        if n < 0:
+            raise RuntimeError("llmgen_blocks_compact failed")
+        for t in tables:
+            a = self._array(t)
+            if L().llmgen_blocks_remap(a, len(t), src, dst, n) != 0:
+                raise RuntimeError("llmgen_blocks_remap failed")
+            t[:] = a[:len(t)]
+        return np.array(src[:n], np.int32), np.array(dst[:n], np.int32)
+
+    def destroy(self) -> None:
+        if self.h:
+            L().llmgen_blocks_destroy(self.h)
+            self.h = None
 
 
 class Graphs:

@@ -28,6 +28,7 @@ from . import attention as A
 from . import host as Hx
 from . import step as stepmod
 from ._lib import lib
+from .cache import BlockCopies, attn_work
 
 
 @dataclass(frozen=True)
@@ -45,6 +46,10 @@ class Qwen3Config:
     rope_theta: float = 1_000_000.0
     max_model_len: int = 1024
     block_size: int = 16  # memory/page_atten.zig:12 PAGE_BLOCK_SIZE
+    # forms of the cache the reference does not have (include/llmgen_cache.h)
+    kv4: bool = False  # pages held in 4 bits
+    window: int = 0  # > 0: rows see the last `window` positions and the first `sinks` ones
+    sinks: int = 0
 
 
 def weight_shapes(cfg: Qwen3Config) -> Dict[str, tuple]:
@@ -129,8 +134,11 @@ class Qwen3:
         self.cos, self.sin = _bits(cos_t, device), _bits(sin_t, device)
         self.max_blocks = (cfg.max_model_len + cfg.block_size - 1) // cfg.block_size
         # paged KV pools, one pair per layer (memory/page_atten.zig:15-28)
-        self.kv = [A.PagedAttentionManager().reserve_layer(i, num_blocks, cfg.n_kv_head, cfg.block_size,
-                                                           cfg.head_dim, device) for i in range(cfg.n_layers)]
+        work = attn_work(device) if cfg.kv4 or cfg.window else None
+        self.kv = [A.PagedAttentionManager().reserve_layer(i, num_blocks, cfg.n_kv_head, cfg.block_size, cfg.head_dim,
+                                                           device, kv4=cfg.kv4, window=cfg.window, sinks=cfg.sinks,
+                                                           work=work) for i in range(cfg.n_layers)]
+        self._copies = BlockCopies([p for kv in self.kv for p in (kv.k, kv.v)])
         self.pf_tile = self.L.hip_attn_prefill_tile()
         # executor.zig:92-102 Workspace.of: metadata, split-K scratch, sampling scratch
         ws = Hx.workspace(cfg.n_head, cfg.head_dim, max_seqs, max_tokens, cfg.max_model_len, cfg.block_size,
@@ -142,6 +150,18 @@ class Qwen3:
         self.sample_scratch = torch.empty(max(ws["sample"], 4), dtype=u8, device=device)
         self.max_seqs, self.max_tokens = max_seqs, max_tokens
         self.step_seed = 0
+
+    def copy_blocks(self, src, dst) -> None:
+        """Copies pages src[i] onto pages dst[i] in every layer's pools (a forked sequence's page about to be written, a
+        compaction; the pairs come from :class:`~llmgen_amd.host.Blocks`)."""
+        self._copies.run(src, dst)
+
+    def _attention(self, g, layer, out, q, k, v, store_kv):
+        kv = self.kv[layer]
+        if kv.form is None:
+            Hx.paged_attention(g, out, q, k, v, kv.k, kv.v, store_kv=store_kv)
+        else:
+            Hx.paged_attention_form(g, kv.form, out, q, k, v, kv.k, kv.v, store_kv=store_kv)
 
     def execute(self, entries: Sequence[stepmod.Entry], ids: Sequence[int], temps=None) -> List[int]:
         """executor.zig:986-1043: a step larger than max_tokens runs as several passes (an entry's query range may
@@ -171,6 +191,13 @@ class Qwen3:
                     out[owner] = tk
         return out
 
+    def _norm_rope(self, q, k, w, g, T):
+        """Per-head RMSNorm and RoPE of q and k, in place."""
+        cfg, L = self.cfg, self.L
+        for x, n, name in ((q, cfg.n_head, "attn_q_norm"), (k, cfg.n_kv_head, "attn_k_norm")):
+            L.hip_rmsnorm(x.data_ptr(), x.data_ptr(), w(name), T * n, cfg.head_dim, cfg.rms_eps)
+            L.hip_rope(x.data_ptr(), x.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(), g.pos, T, n, cfg.head_dim)
+
     # -- buffers of one step
     def _empty(self, *shape, dtype=torch.int16):
         return torch.empty(shape, dtype=dtype, device=self.device)
@@ -183,7 +210,8 @@ class Qwen3:
         layer in nine launches: the projections of one input together (hip_linear3), q/k norm + RoPE + the KV write
         as one kernel (hip_qk_norm_rope_store_kv), the residual adds with the product before them (hip_linear_add)
         and SiLU with the product after it (hip_silu_mul); without it the reference graph's launches run one by one.
-        Both give identical values."""
+        Both give identical values.  4-bit pages have no fused KV write: q/k norm, RoPE and the write are launches of
+        their own."""
         cfg, L = self.cfg, self.L
         T, S = sum(e.q_len for e in entries), len(entries)
         if len(ids) != T or T > self.max_tokens or S > self.max_seqs:
@@ -232,10 +260,14 @@ class Qwen3:
             if fused_qk:
                 L.hip_linear3(p(q), w("attn_q"), nq * hd, p(k), w("attn_k"), nkv * hd, p(v), w("attn_v"), nkv * hd,
                               p(xn), T, H)
-                L.hip_qk_norm_rope_store_kv(p(q), p(kv.k), p(kv.v), p(q), p(k), p(v), w("attn_q_norm"),
-                                            w("attn_k_norm"), cfg.rms_eps, p(self.cos), p(self.sin), g.pos, g.slots,
-                                            T, nq, nkv, hd, cfg.block_size)
-                Hx.paged_attention(g, attn, q, k, v, kv.k, kv.v, store_kv=False)
+                if cfg.kv4:
+                    self._norm_rope(q, k, w, g, T)
+                    self._attention(g, i, attn, q, k, v, True)
+                else:
+                    L.hip_qk_norm_rope_store_kv(p(q), p(kv.k), p(kv.v), p(q), p(k), p(v), w("attn_q_norm"),
+                                                w("attn_k_norm"), cfg.rms_eps, p(self.cos), p(self.sin), g.pos, g.slots,
+                                                T, nq, nkv, hd, cfg.block_size)
+                    self._attention(g, i, attn, q, k, v, False)
                 L.hip_linear_add(p(x), p(x), p(attn), w("attn_output"), T, H, nq * hd)
                 L.hip_rmsnorm(p(xn), p(x), w("ffn_norm"), T, H, cfg.rms_eps)
                 L.hip_linear3(p(gate), w("ffn_gate"), F, p(up), w("ffn_up"), F, None, None, 0, p(xn), T, H)
@@ -245,11 +277,8 @@ class Qwen3:
                 L.hip_linear(p(q), 0, p(xn), w("attn_q"), T, nq * hd, H)
                 L.hip_linear(p(k), 0, p(xn), w("attn_k"), T, nkv * hd, H)
                 L.hip_linear(p(v), 0, p(xn), w("attn_v"), T, nkv * hd, H)
-                L.hip_rmsnorm(p(q), p(q), w("attn_q_norm"), T * nq, hd, cfg.rms_eps)
-                L.hip_rmsnorm(p(k), p(k), w("attn_k_norm"), T * nkv, hd, cfg.rms_eps)
-                L.hip_rope(p(q), p(q), p(self.cos), p(self.sin), g.pos, T, nq, hd)
-                L.hip_rope(p(k), p(k), p(self.cos), p(self.sin), g.pos, T, nkv, hd)
-                Hx.paged_attention(g, attn, q, k, v, kv.k, kv.v)
+                self._norm_rope(q, k, w, g, T)
+                self._attention(g, i, attn, q, k, v, True)
                 L.hip_linear(p(o), 0, p(attn), w("attn_output"), T, H, nq * hd)
                 L.hip_add(p(x), p(x), p(o), T * H)
                 L.hip_rmsnorm(p(xn), p(x), w("ffn_norm"), T, H, cfg.rms_eps)
