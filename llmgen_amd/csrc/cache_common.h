@@ -30,6 +30,21 @@ __device__ __forceinline__ u32x4_t kv4_to_bf16(uint32_t w, float scale) {
 // the f32 whose exponent field is scale byte b (0 gives the subnormal field that the conversion reads as 2^-127)
 __device__ __forceinline__ float kv4_scale(uint32_t b) { return __builtin_bit_cast(float, b << 23); }
 
+// Division of a token's position by the block size: a shift for a power of two, else a multiplication by
+// floor(2^32 / bs), which falls short by at most one for positions below 2^30.
+struct PageDiv {
+    int bs, shift;
+    uint32_t magic;
+    __device__ __forceinline__ int operator()(int t) const {
+        if (shift >= 0) return t >> shift;
+        const int d = (int)__umulhi((uint32_t)t, magic);
+        return t - d * bs >= bs ? d + 1 : d;
+    }
+};
+inline PageDiv page_div(int bs) {
+    return PageDiv{bs, (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1, bs > 1 ? (uint32_t)((1ull << 32) / bs) : 0u};
+}
+
 // No window is a window longer than any sequence, so that the kernels know one rule only.
 constexpr int NO_WINDOW = 1 << 30;
 

@@ -111,8 +111,8 @@ bool check_rows(const char *who, const void *k, const void *v, const void *slots
 // ------------------------------------------------------------------------------------------------------------
 // Split-K decode
 // ------------------------------------------------------------------------------------------------------------
-// One workgroup of 4 waves takes a span of one (sequence, kv head)'s visible keys, in tiles of 16 keys; a wave takes NT
-// tiles (NT * 16 keys, 8.5 KB of codes and scales at NT = 4) a round and works alone until the end.
+// One workgroup of 4 or 8 waves takes a span of one (sequence, kv head)'s visible keys, in tiles of 16 keys; a wave takes
+// NT tiles (64 keys, 8.5 KB of codes and scales) a round and works alone until the end.
 //   * K: lane (row l % 16, run l / 16) loads the 16 bytes that hold 32 values of one key, so a tile is one contiguous
 //     kilobyte in one access, and converts them to four A fragments of v_mfma_f32_16x16x32_bf16 in registers.  Step c of
 //     the product takes values 8c..8c+7 of every run; q is loaded in the same order, so no lane exchange is needed.
@@ -128,10 +128,11 @@ bool check_rows(const char *who, const void *k, const void *v, const void *slots
 //   * The loads of a round are issued when the registers they go to were just converted, a round ahead of their use.
 // The waves' (m, l, O) are merged through LDS; a sequence with several spans leaves them in the caller's scratch, and
 // the last workgroup of the (sequence, kv head) to finish merges them, by a counter that returns to 0.
-constexpr int NW = 4;         // waves a workgroup
-constexpr int TILE = 16;      // keys a tile
+constexpr int TILE = 16;  // keys a tile
+constexpr int NT = 4;     // tiles a wave takes a round
 constexpr int MAX_PARTS = 256;  // spans a sequence: their weights for 16 heads fill the 32 KB of LDS when merging
 
+template <int NW>
 struct DecodeLds {
     __attribute__((aligned(16))) unsigned char v[NW][32 * HD * 2];
     float m[NW][16];
@@ -145,10 +146,14 @@ __device__ __forceinline__ s16x4_t ds_read_tr(const bf16_t *p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)p);
 }
 
-// maximum / sum over the four lanes l % 16 of a wave's 16-lane groups
+// maximum / sum over the four lanes l % 16 of a wave's 16-lane groups: swap the halves of every 32 lanes, then of 64
 __device__ __forceinline__ float group_max(float x) {
-    x = fmaxf(x, lane_xor(x, 16));
-    return fmaxf(x, lane_xor(x, 32));
+    auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t a = r[0], b = r[1];
+    x = fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    auto t = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t c = t[0], d = t[1];
+    return fmaxf(__builtin_bit_cast(float, c), __builtin_bit_cast(float, d));
 }
 __device__ __forceinline__ float group_sum(float x) {
     x += lane_xor(x, 16);
@@ -159,17 +164,16 @@ __device__ __forceinline__ u32x4_t ld16_stream(const void *p) {
     return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(p));
 }
 
-// PAGE16: block_size % 16 == 0, a tile lies inside one page (one block-table read a tile, in scalar registers); else
-// each lane looks its own key's page up.
-template <bool PAGE16, int NT>
+// PAGE16: block_size % 16 == 0, a tile lies inside one page; else each lane looks its own key's page up.
+template <bool PAGE16, int NW>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)))
     attn_decode_kv4_kernel(bf16_t *__restrict__ out, const bf16_t *__restrict__ q, const uint8_t *__restrict__ kc,
                            const uint8_t *__restrict__ vc, const int *__restrict__ block_tables,
                            const int *__restrict__ ctx_lens, const int *__restrict__ cu_q,
                            const int *__restrict__ tile_seq, int S, int nq, int nkv, int G, int max_blocks,
-                           int block_size, int bs_shift, float scale_log2, int window, int sinks, int span0, int nparts,
+                           PageDiv div, float scale_log2, int window, int sinks, int span0, int nparts,
                            float *__restrict__ part_o, float *__restrict__ part_ml, int *__restrict__ counters) {
-    __shared__ DecodeLds sm;
+    __shared__ DecodeLds<NW> sm;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, rgrp = lane >> 4;
     const int kvh = blockIdx.x % nkv;
@@ -183,6 +187,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)
         row = cu_q[s];
         if (cu_q[s + 1] - row != 1) return;
     }
+    const int block_size = div.bs;
     const int ctx = (int)min((long)ctx_lens[s], (long)max_blocks * block_size);
     if (ctx <= 0) {
         if (part == 0)
@@ -231,53 +236,82 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)
         ksc[i] = vsc[i] = 0;
     }
     auto tile_key = [&](int vt) { return vt * TILE + (vt >= st ? gap : 0); };
-    auto seen = [&](int t) { return t < ctx && (t >= lo || t < sinks); };
-    // byte offset of key t's codes and scales in the pool; a key that is not visible is replaced by one that is
-    auto place = [&](int t, long &codes, long &scales) {
-        t = min(t, ctx - 1);
-        if (t >= sinks && t < lo) t = lo;
-        const int blk = bs_shift >= 0 ? t >> bs_shift : t / block_size;
-        const int off = t - blk * block_size;
+    auto hidden = [&](int t) -> bool { return (t >= ctx) | ((t < lo) & (t >= sinks)); };  // no branches
+    // Pages are looked up ahead of use.  PAGE16: lane l holds the place of tile l % NT of round l / NT of the next AHEAD
+    // rounds (looked up together, one load), read out as scalars; a tile past the span's end is its last one, read again
+    // and masked, so that loads need no branch.  Else lanes hold the place of their own keys of the next round; a key
+    // that is not visible is replaced by one that is.
+    constexpr int AHEAD = 64 / NT;
+    long at_codes = 0, at_scales = 0;
+    long kcodes[NT], kscales[NT], vcodes[NT], vscales[NT];
+    auto key_place = [&](int t, long &codes, long &scales) {
+        const int blk = div(t), off = t - blk * block_size;
         const long base = (long)bt[blk] * page;
-        codes = base + (long)off * CODE_BYTES;
-        scales = base + scale_at + (long)off * SCALE_BYTES;
+        codes = base + off * CODE_BYTES;
+        scales = base + scale_at + off * SCALE_BYTES;
     };
-    auto load = [&](const uint8_t *pool, int vt, int r, int run, u32x4_t &x, uint32_t &sc) {
-        if (vt >= t_end) return;  // uniform across the wave
-        const int t0 = tile_key(vt);
-        if (PAGE16) {
-            const int blk = bs_shift >= 0 ? t0 >> bs_shift : t0 / block_size;
-            const int off = t0 - blk * block_size;
-            const uint8_t *p = pool + (long)bt[blk] * page + (long)off * CODE_BYTES;
-            const uint8_t *ps = pool + (long)bt[blk] * page + scale_at + off * SCALE_BYTES;
-            x = ld16_stream(p + r * CODE_BYTES + run * 16);
-            sc = ps[r * SCALE_BYTES + run];
+    auto lookup = [&](int vt0, int r) {  // for round r of the wave, whose first tile is vt0
+        if constexpr (PAGE16) {
+            if (r % AHEAD == 0)
+                key_place(tile_key(min(vt0 + (lane / NT) * NW * NT + lane % NT, t_end - 1)), at_codes, at_scales);
         } else {
-            long codes, scales;
-            place(t0 + r, codes, scales);
-            x = ld16_stream(pool + codes + run * 16);
-            sc = pool[scales + run];
+            auto some = [&](int t) {
+                t = min(t, ctx - 1);
+                return t >= sinks && t < lo ? lo : t;
+            };
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const int t0 = tile_key(min(vt0 + i, t_end - 1));
+                key_place(some(t0 + col), kcodes[i], kscales[i]);
+                key_place(some(t0 + (lane >> 2)), vcodes[i], vscales[i]);
+            }
         }
     };
-    auto load_k = [&](int vt0) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) load(kbase, vt0 + i, col, rgrp, kreg[i], ksc[i]);
+    auto scalar = [](long x, int l) {
+        const uint32_t a = __builtin_amdgcn_readlane((int)x, l), b = __builtin_amdgcn_readlane((int)(x >> 32), l);
+        return (long)((uint64_t)b << 32 | a);
     };
-    auto load_v = [&](int vt0) {
+    const int k_at = col * CODE_BYTES + rgrp * 16, ks_at = col * SCALE_BYTES + rgrp;
+    auto load_k = [&](int r) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) load(vbase, vt0 + i, lane >> 2, lane & 3, vreg[i], vsc[i]);
+        for (int i = 0; i < NT; ++i) {
+            if constexpr (PAGE16) {
+                const int l = r % AHEAD * NT + i;
+                kreg[i] = ld16_stream(kbase + scalar(at_codes, l) + k_at);
+                ksc[i] = (kbase + scalar(at_scales, l))[ks_at];
+            } else {
+                kreg[i] = ld16_stream(kbase + kcodes[i] + rgrp * 16);
+                ksc[i] = kbase[kscales[i] + rgrp];
+            }
+        }
+    };
+    auto load_v = [&](int r) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            if constexpr (PAGE16) {
+                const int l = r % AHEAD * NT + i;
+                vreg[i] = ld16_stream(vbase + scalar(at_codes, l) + lane * 16);
+                vsc[i] = (vbase + scalar(at_scales, l))[lane];
+            } else {
+                vreg[i] = ld16_stream(vbase + vcodes[i] + (lane & 3) * 16);
+                vsc[i] = vbase[vscales[i] + (lane & 3)];
+            }
+        }
     };
 
     bf16_t *vl = reinterpret_cast<bf16_t *>(sm.v[wave]);
     int vt0 = part * span + wave * NT;
     if (vt0 < t_end) {
-        load_k(vt0);
-        load_v(vt0);
+        lookup(vt0, 0);
+        load_k(0);
+        load_v(0);
+        if (!PAGE16 && vt0 + NW * NT < t_end) lookup(vt0 + NW * NT, 1);
     }
-    for (; vt0 < t_end; vt0 += NW * NT) {
+    for (int r = 0; vt0 < t_end; vt0 += NW * NT, ++r) {
         const int next = vt0 + NW * NT;
+        if (PAGE16 && next < t_end) lookup(next, r + 1);
         // ---- scores ----
-        f32x4_t sc[NT];
+        float sc[NT][4];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const float s2 = kv4_scale(ksc[i]);
@@ -286,70 +320,92 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)
             for (int c = 0; c < 4; ++c)
                 acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kv4_to_bf16(kreg[i][c], s2)),
                                                               qf[c], acc, 0, 0, 0);
-            sc[i] = acc;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[i][j] = acc[j];
         }
-        if (next < t_end) load_k(next);
-        float mx = -INFINITY;
+        if (next < t_end) load_k(r + 1);
+        // a round is visible as a whole except at the ends of the sinks, the window and the sequence (uniform)
+        const int first = tile_key(vt0), end = tile_key(vt0 + NT - 1) + TILE;
+        if (!(vt0 + NT <= t_end && end <= ctx && (vt0 >= st ? first >= lo : end <= sinks))) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int t0 = tile_key(vt0 + i);
-            // whole tiles are visible except at the ends of the sinks, the window and the sequence (uniform)
-            const bool whole = vt0 + i < t_end && t0 + TILE <= ctx && (t0 >= lo || t0 + TILE <= sinks);
+            for (int i = 0; i < NT; ++i) {
+                const int t0 = tile_key(vt0 + i);
+                const bool out_of_span = vt0 + i >= t_end;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sc[i][j] *= scale_log2;
-                if (!whole && !(vt0 + i < t_end && seen(t0 + rgrp * 4 + j))) sc[i][j] = -INFINITY;
-                mx = fmaxf(mx, sc[i][j]);
+                for (int j = 0; j < 4; ++j)
+                    sc[i][j] = (out_of_span | hidden(t0 + rgrp * 4 + j)) ? -INFINITY : sc[i][j];
+                // finite values behind a probability of 0
+                vsc[i] = (out_of_span | hidden(t0 + (lane >> 2))) ? 0 : vsc[i];
             }
-            if (!whole && !seen(t0 + (lane >> 2))) vsc[i] = 0;  // finite values behind a probability of 0
         }
-        // ---- online softmax of head col ----
-        mx = group_max(mx);
-        const float m_new = fmaxf(m_run, mx);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        if (__any(m_new > m_run)) {
+        // ---- online softmax of head col.  Once every head has a reference m_run, probabilities are taken against it
+        //      without a maximum (they may exceed 1: o / l is unchanged by a common factor); only a sum beyond 2^64 moves
+        //      the reference ----
+        u32x2_t p[NT];
+        float lsum;
+        auto probs = [&](float m_use) {
+            lsum = 0.f;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                float e[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    e[j] = fast_exp2(__builtin_fmaf(sc[i][j], scale_log2, -m_use));
+                    lsum += e[j];
+                }
+                p[i] = u32x2_t{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
+            }
+        };
+        bool move = !__all(m_run > -INFINITY);
+        if (!move) {
+            probs(m_run);
+            move = __any(!(lsum <= 0x1p64f));
+        }
+        if (move) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mx = fmaxf(mx, sc[i][j]);
+            const float m_new = fmaxf(m_run, group_max(mx) * scale_log2);  // scale > 0 commutes with the maximum
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
             const float corr = fast_exp2(m_run - m_use);
             l_run *= corr;
 #pragma unroll
             for (int db = 0; db < 8; ++db)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[db][j] *= corr;
+            m_run = m_new;
+            probs(m_use);
         }
-        m_run = m_new;
-        u32x2_t p[NT];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            float e[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                e[j] = fast_exp2(sc[i][j] - m_use);
-                l_run += e[j];
-            }
-            p[i] = u32x2_t{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
-        }
+        l_run += lsum;
         // ---- O^T += V^T P^T, two tiles (32 keys) a step ----
 #pragma unroll
         for (int h = 0; h < NT / 2; ++h) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float s2 = kv4_scale(vsc[2 * h + i]);
-                const int r = i * 16 + (lane >> 2);
+                const int lr = i * 16 + (lane >> 2);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int chunk = ((lane & 3) * 4 + c) ^ ((r & 7) << 1);
-                    *reinterpret_cast<u32x4_t *>(vl + r * HD + chunk * 8) = kv4_to_bf16(vreg[2 * h + i][c], s2);
+                    const int chunk = ((lane & 3) * 4 + c) ^ ((lr & 7) << 1);
+                    *reinterpret_cast<u32x4_t *>(vl + lr * HD + chunk * 8) = kv4_to_bf16(vreg[2 * h + i][c], s2);
                 }
+            }
+            if (h == NT / 2 - 1 && next < t_end) {
+                load_v(r + 1);
+                if (!PAGE16 && next + NW * NT < t_end) lookup(next + NW * NT, r + 2);
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
             const u32x4_t pw = {p[2 * h][0], p[2 * h][1], p[2 * h + 1][0], p[2 * h + 1][1]};
             const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, pw);
-            const int r = rgrp * 4 + (col >> 2);  // this lane's row of a transposed read, in either tile
+            const int tr = rgrp * 4 + (col >> 2);  // this lane's row of a transposed read, in either tile
 #pragma unroll
             for (int db = 0; db < 8; ++db) {
-                const int chunk = (db * 2 + ((col & 3) >> 1)) ^ ((r & 7) << 1);
-                const bf16_t *src = vl + r * HD + chunk * 8 + (col & 1) * 4;
+                const int chunk = (db * 2 + ((col & 3) >> 1)) ^ ((tr & 7) << 1);
+                const bf16_t *src = vl + tr * HD + chunk * 8 + (col & 1) * 4;
                 const s16x4_t a0 = ds_read_tr(src), a1 = ds_read_tr(src + 16 * HD);
                 o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                     __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7)), pb, o[db], 0, 0,
@@ -360,7 +416,6 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
-        if (next < t_end) load_v(next);
     }
 
     // ---- merge the waves ----
@@ -453,15 +508,18 @@ struct DecodeShape {
 };
 
 void launch_decode(bf16_t *out, const bf16_t *q, const uint8_t *kc, const uint8_t *vc, const int *bt, const int *ctx,
-                   const int *cu_q, const int *tile_seq, const DecodeShape &d, int span, int nparts, const Work &w) {
-    constexpr int NT = 4;
-    const int bs_shift = (d.block_size & (d.block_size - 1)) == 0 ? __builtin_ctz(d.block_size) : -1;
+                   const int *cu_q, const int *tile_seq, const DecodeShape &d, int span, int nparts, const Work &w,
+                   int waves) {
     const long rows = (long)d.S * d.nq * nparts;
     float *part_o = nparts > 1 ? w.part : nullptr, *part_ml = nparts > 1 ? w.part + rows * HD : nullptr;
-    auto kern = d.block_size % TILE == 0 ? attn_decode_kv4_kernel<true, NT> : attn_decode_kv4_kernel<false, NT>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)((long)d.nkv * d.S * nparts)), dim3(64 * NW), 0, g_llmgen_stream, out, q, kc,
-                       vc, bt, ctx, cu_q, tile_seq, d.S, d.nq, d.nkv, d.G, d.max_blocks, d.block_size, bs_shift, d.sl2,
-                       d.window, d.sinks, span, nparts, part_o, part_ml, w.counters);
+    auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, dim3((unsigned)((long)d.nkv * d.S * nparts)), dim3(64 * waves), 0, g_llmgen_stream, out, q,
+                           kc, vc, bt, ctx, cu_q, tile_seq, d.S, d.nq, d.nkv, d.G, d.max_blocks, page_div(d.block_size),
+                           d.sl2, d.window, d.sinks, span, nparts, part_o, part_ml, w.counters);
+    };
+    const bool page16 = d.block_size % TILE == 0;
+    if (waves == 8) go(page16 ? attn_decode_kv4_kernel<true, 8> : attn_decode_kv4_kernel<false, 8>);
+    else go(page16 ? attn_decode_kv4_kernel<true, 4> : attn_decode_kv4_kernel<false, 4>);
 }
 
 }  // namespace
@@ -500,21 +558,35 @@ extern "C" void hip_attn_decode_kv4(bf16_t *out, const bf16_t *q, const uint8_t 
     DecodeShape d{S, nq, nkv, nq / nkv, max_blocks, block_size, scale * LLMGEN_LOG2E,
                   window ? std::min(window, NO_WINDOW) : NO_WINDOW, std::min(sinks, NO_WINDOW)};
     const Work w = split_work(work, work_bytes);
-    // Tiles of the longest expected sequence, and spans so that the launch has about four workgroups a CU; a span is at
-    // least one round of the four waves.
+    // How the keys are split, measured over 1 to 200 sequences of 300 to 32768 keys: about 8 waves a CU in all, and as
+    // few spans as that allows, since each span more is one more partial result to merge (32 sequences x 8 heads of 1024
+    // keys: one span of 8 waves 9.4 us, two of 4 waves 18 us).
+    //   * enough (sequence, KV head) pairs for the chip: one span, of 8 waves up to two pairs a CU (256 pairs x 1024
+    //     keys 9.4 us against 11.5 us with 4), of 4 above (512 pairs x 700 keys 11.8 against 14.5 us);
+    //   * fewer pairs: spans of at least one round of their waves; 4 waves, or 8 where that would be more than 8 spans (8
+    //     pairs x 32768 keys: 32 spans of 8 waves 16.0 us, 32 of 4 19.4, 64 of 4 24 us; 8 pairs x 2048 keys: 8 spans of 4
+    //     waves 8.4 us, 4 of 8 9.6 us);
+    //   * at most one round of 8 waves: one span (8 pairs x 512 keys 6.4 us against 7.7 us split).
     long keys = std::max(1, std::min(max_ctx, max_blocks * block_size));
     keys = std::min(keys, (long)d.window + d.sinks + 2 * TILE);
-    const long tiles = (keys + TILE - 1) / TILE;
-    constexpr int ROUND = NW * 4;
-    long parts = std::min<long>({(4L * llmgen_num_cus() + (long)S * nkv - 1) / ((long)S * nkv),
-                                 (tiles + ROUND - 1) / ROUND, MAX_PARTS, w.floats / ((long)S * nq * (HD + 2))});
-    if (parts < 1 || (long)S * nkv > WORK_COUNTERS) parts = 1;
-    const long span = ((tiles + parts - 1) / parts + 3) / 4 * 4;
-    if ((long)nkv * S * parts > 0x7fffffffL) {
+    const long tiles = (keys + TILE - 1) / TILE, pairs = (long)S * nkv, cus = llmgen_num_cus();
+    int waves = 8;
+    long parts = 1;
+    if (pairs >= 2 * cus) {
+        waves = 4;
+    } else if (pairs < cus && tiles > 8 * NT) {
+        parts = std::min((2 * cus + pairs - 1) / pairs, (tiles + 4 * NT - 1) / (4 * NT));
+        if (parts > 8) parts = (parts + 1) / 2;
+        else waves = 4;
+    }
+    parts = std::min<long>({parts, MAX_PARTS, w.floats / ((long)S * nq * (HD + 2))});
+    if (parts < 1 || pairs > WORK_COUNTERS) parts = 1;
+    const long span = ((tiles + parts - 1) / parts + NT - 1) / NT * NT;
+    if (pairs * parts > 0x7fffffffL) {
         refuse(who, "too many sequences");
         return;
     }
-    launch_decode(out, q, k_cache, v_cache, block_tables, ctx_lens, nullptr, nullptr, d, (int)span, (int)parts, w);
+    launch_decode(out, q, k_cache, v_cache, block_tables, ctx_lens, nullptr, nullptr, d, (int)span, (int)parts, w, waves);
 }
 
 // The single rows of a prefill step over 4-bit pages: one workgroup a (row, kv head).
@@ -523,5 +595,5 @@ void llmgen_kv4_rows_of_prefill(bf16_t *out, const bf16_t *q, const uint8_t *k_c
                                 int n_tiles, int nq, int nkv, int max_blocks, int block_size, float scale_log2, int window,
                                 int sinks) {
     DecodeShape d{n_tiles, nq, nkv, nq / nkv, max_blocks, block_size, scale_log2, window, sinks};
-    launch_decode(out, q, k_cache, v_cache, block_tables, ctx_lens, cu_q, tile_seq, d, 1 << 26, 1, Work{});
+    launch_decode(out, q, k_cache, v_cache, block_tables, ctx_lens, cu_q, tile_seq, d, 1 << 26, 1, Work{}, 4);
 }

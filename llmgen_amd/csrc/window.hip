@@ -76,7 +76,9 @@ void launch_rows_g(const RowArgs &a, int waves) {
 // ------------------------------------------------------------------------------------------------------------
 // Prefill
 // ------------------------------------------------------------------------------------------------------------
-constexpr int PIECES_MAX = 8, PIECE_MIN_TILES = 4;
+// Pieces a unit, and key tiles a piece has at least.  Up to 16 pieces: 100 rows behind 8000 keys, 16 units, 48.6 us with
+// 8 and 40.2 us with 16, though the merge reads 68 KB a piece.
+constexpr int PIECES_MAX = 16, PIECE_MIN_TILES = 4;
 
 template <int NW, int MODE>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
@@ -84,43 +86,42 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)
                                int *__restrict__ counters) {
     using namespace llmgen_window;
     __shared__ __attribute__((aligned(16))) unsigned char lds[sizeof(WindowLds<NW>)];
-    if constexpr (NW <= 4) {
-        if (P > 1) {
-            __shared__ int s_last;
-            const int unit = (int)(blockIdx.x % n_units), piece = (int)(blockIdx.x / n_units);
-            const int tile = a.n_tiles - 1 - unit / (a.nkv * a.head_groups);
-            const int s = a.tile_seq[tile], q0 = a.tile_q0[tile], q_len = a.cu_q[s + 1] - a.cu_q[s];
-            const int ctx = (int)min((long)a.ctx_lens[s], (long)a.max_blocks * a.block_size);
-            const int n = (q_len > 1 || a.single) && ctx >= q_len
-                              ? key_tiles(ctx - q_len + q0, ctx - q_len + min(q0 + BQ, q_len), a.window, a.sinks).n
-                              : 0;
-            const int pe = n < 2 ? 1 : min(P, (n + PIECE_MIN_TILES - 1) / PIECE_MIN_TILES);
-            if (piece >= pe) return;
-            if (pe > 1) {
-                constexpr int PSTRIDE = NW * PART_WAVE_FLOATS;
-                float *base = part + (long)unit * P * PSTRIDE;
-                window_body<NW, MODE>(a, unit, lds, (int)((long)piece * n / pe), (int)((long)(piece + 1) * n / pe),
-                                      base + (long)piece * PSTRIDE);
-                // publish (device-coherent stores, complete before the barrier), then draw a ticket: the last merges
-                __builtin_amdgcn_s_waitcnt(0);
-                __syncthreads();
-                if (threadIdx.x == 0)
-                    s_last = __hip_atomic_fetch_add(counters + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                             pe - 1;
-                __syncthreads();
-                if (!s_last) return;
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-                prefill_merge_store_n<PIECES_MAX, NW>(a.out, a.cu_q, a.tile_seq, a.tile_q0, a.n_tiles, a.nq, a.nkv, a.G,
-                                                      a.head_groups, unit, base, pe);
-                if (threadIdx.x == 0)
-                    __hip_atomic_store(counters + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                return;
-            }
-            window_body<NW, MODE>(a, unit, lds, 0, -1, nullptr);
-            return;
+    __shared__ int s_last;
+    const int unit = (int)(blockIdx.x % n_units), piece = (int)(blockIdx.x / n_units);
+    int pe = 1, j0 = 0, j1 = -1;
+    constexpr int PSTRIDE = NW * PART_WAVE_FLOATS;
+    float *base = nullptr;
+    if (NW <= 4 && P > 1) {  // which share of the unit's key tiles
+        const int tile = a.n_tiles - 1 - unit / (a.nkv * a.head_groups);
+        const int s = a.tile_seq[tile], q0 = a.tile_q0[tile], q_len = a.cu_q[s + 1] - a.cu_q[s];
+        const int ctx = (int)min((long)a.ctx_lens[s], (long)a.max_blocks * a.block_size);
+        const int n = (q_len > 1 || a.single) && ctx >= q_len
+                          ? key_tiles(ctx - q_len + q0, ctx - q_len + min(q0 + BQ, q_len), a.window, a.sinks).n
+                          : 0;
+        pe = n < 2 ? 1 : min(P, (n + PIECE_MIN_TILES - 1) / PIECE_MIN_TILES);
+        if (piece >= pe) return;
+        if (pe > 1) {
+            base = part + (long)unit * P * PSTRIDE;
+            j0 = (int)((long)piece * n / pe);
+            j1 = (int)((long)(piece + 1) * n / pe);
         }
     }
-    window_body<NW, MODE>(a, blockIdx.x, lds, 0, -1, nullptr);
+    float *mine = base ? base + (long)piece * PSTRIDE : nullptr;
+    window_body<NW, MODE>(a, unit, lds, j0, j1, mine);
+    if constexpr (NW <= 4) {
+        if (pe == 1) return;
+        // publish (device-coherent stores, complete before the barrier), then draw a ticket: the last merges
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (threadIdx.x == 0)
+            s_last = __hip_atomic_fetch_add(counters + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == pe - 1;
+        __syncthreads();
+        if (!s_last) return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        prefill_merge_store_n<PIECES_MAX, NW>(a.out, a.cu_q, a.tile_seq, a.tile_q0, a.n_tiles, a.nq, a.nkv, a.G,
+                                              a.head_groups, unit, base, pe);
+        if (threadIdx.x == 0) __hip_atomic_store(counters + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
 }
 
 template <int NW>
@@ -167,9 +168,15 @@ void prefill(const char *who, bool kv4, bf16_t *out, const bf16_t *q, const void
     if (busy > 0 && busy * 2 <= slots && units <= WORK_COUNTERS)
         P = std::min<long>({PIECES_MAX, slots / busy, w.floats / (units * nw * PART_WAVE_FLOATS)});
     if (P < 1) P = 1;
-    if (P == 1 && G >= 4) {
+    // Four heads a workgroup read each K/V tile once for all of them, two heads leave two workgroups a CU that hide each
+    // other's start and end: 16384 rows x 32 heads with a window of 256 keys 199 -> 169 us with two, of 1024 365 -> 353
+    // us, of 4096 432 -> 439 us (pages whose tiles take several DMA descriptors: 192 -> 181, 382 -> 399 us).  Steps of at
+    // most one four-head unit a CU want the smaller ones too (a prompt of 2048 tokens 67.7 -> 57.8 us).
+    const int short_window = mode == DMA_ROW4 || mode == DMA_FLAT ? 512 : 2048;
+    const long units8 = (long)n_tiles * nkv * (G / 4);
+    if (P == 1 && G >= 4 && window > short_window && units8 > llmgen_num_cus()) {
         nw = 8;
-        units = (long)n_tiles * nkv * (G / 4);
+        units = units8;
     }
     if (units * P > 0x7fffffffL || (long)n_tiles * nkv > 0x7fffffffL) {
         refuse(who, "too many tiles");

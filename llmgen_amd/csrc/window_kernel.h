@@ -63,9 +63,100 @@ struct WindowArgs {
     bool single;  // segments of one row are computed here (no decode launch for them)
 };
 
+// One query row (at element `row` of q and out, position pos) over n tiles from j0 on, by one wave: lane = key for the
+// scores, lane = two values of the head for the sums, online softmax in base 2.  Reads only keys that the row sees.  The
+// result goes to out, or as row r of a wave's partial result.
+template <int MODE>
+__device__ __forceinline__ void redo_row(const WindowArgs &a, const int *bt, int kvh, long row, int pos, const KeyTiles &kt,
+                                         int j0, int n, float *part, int r) {
+    const int lane = threadIdx.x & 63;
+    const long hb = MODE == KV4 ? llmgen_cache::head_bytes(a.block_size) : (long)a.block_size * HD * 2;
+    auto place = [&](int t, int &off) {  // key t's page and head, and its row there
+        const int blk = t / a.block_size;
+        off = t - blk * a.block_size;
+        return ((long)bt[blk] * a.nkv + kvh) * hb;
+    };
+    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        const int ti = j0 + i, kb0 = (ti >= kt.sink_tiles ? ti + kt.gap : ti) * BK, t = kb0 + lane;
+        const bool vis = t <= pos && (t > pos - a.window || t < a.sinks);
+        float s = -INFINITY;
+        if (vis) {
+            int off;
+            const uint8_t *p = static_cast<const uint8_t *>(a.kc) + place(t, off);
+            s = 0.f;
+#pragma unroll 1
+            for (int run = 0; run < 4; ++run) {
+                u32x4_t codes;
+                float sc = 0.f;
+                if (MODE == KV4) {
+                    codes = ld16(p + (long)off * llmgen_cache::CODE_BYTES + run * 16);
+                    sc = llmgen_cache::kv4_scale(p[(long)a.block_size * llmgen_cache::CODE_BYTES +
+                                                   (long)off * llmgen_cache::SCALE_BYTES + run]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float kf[8], qf[8];
+                    unpack_bf16x8(MODE == KV4 ? llmgen_cache::kv4_to_bf16(codes[c], sc)
+                                              : ld16(p + (long)off * (HD * 2) + run * 64 + c * 16), kf);
+                    unpack_bf16x8(ld16(a.q + row + run * 32 + c * 8), qf);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s = __builtin_fmaf(kf[e], qf[e], s);
+                }
+            }
+            s *= a.scale_log2;
+        }
+        float mx = s;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, lane_xor(mx, d));
+        const float m_new = fmaxf(m, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float corr = fast_exp2(m - m_use), p = fast_exp2(s - m_use);
+        float sum = p;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) sum += lane_xor(sum, d);
+        l = l * corr + sum;
+        o0 *= corr;
+        o1 *= corr;
+        m = m_new;
+        for (uint64_t left = __ballot(vis); left; left &= left - 1) {
+            const int j = __builtin_ctzll(left);
+            const float pj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j));
+            int off;
+            const uint8_t *v = static_cast<const uint8_t *>(a.vc) + place(kb0 + j, off);
+            uint32_t w;
+            if (MODE == KV4) {
+                const uint32_t code = v[(long)off * llmgen_cache::CODE_BYTES + lane];
+                w = llmgen_cache::kv4_to_bf16(code, llmgen_cache::kv4_scale(
+                    v[(long)a.block_size * llmgen_cache::CODE_BYTES + (long)off * llmgen_cache::SCALE_BYTES + lane / 16]))[0];
+            } else {
+                w = *reinterpret_cast<const uint32_t *>(v + (long)off * (HD * 2) + lane * 4);
+            }
+            o0 = __builtin_fmaf(pj, bf16lo_to_f32(w), o0);
+            o1 = __builtin_fmaf(pj, bf16hi_to_f32(w), o1);
+        }
+    }
+    if (!part) {
+        *reinterpret_cast<uint32_t *>(a.out + row + lane * 2) = pack_bf16x2(o0 / l, o1 / l);
+        return;
+    }
+    const int d = lane * 2;  // value d of row r lies at [db * 16 + (d / 8) % 4 * 4 + d % 4][half * 32 + r], half = d / 4 % 2
+    float *at = part + ((d >> 5) * 16 + (d >> 3 & 3) * 4 + (d & 3)) * 64 + (d >> 2 & 1) * 32 + r;
+    __hip_atomic_store(at, o0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(at + 64, o1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (lane < 2) {  // the merge adds the halves' l
+        __hip_atomic_store(part + 64 * 64 + lane * 32 + r, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(part + 65 * 64 + lane * 32 + r, lane ? 0.f : l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+
 // The workgroup's work: unit `bid` of the grid (KV head fastest, then group of NW / 2 heads, then tile from the end of
 // the list), key tiles [j0, j1) of it (j1 < 0: to its last).  If part is not null the partial result goes there
 // (device-coherent stores, NW * PART_WAVE_FLOATS floats, the layout prefill_merge_store_n reads) instead of rows to out.
+//
+// Masking a score does not stop an infinity or NaN in V, as 0 times it is NaN.  Rows whose accumulators end up with one
+// (and whose scores have none: then the result is NaN) are therefore computed again by redo_row, which multiplies only
+// values that the row sees.
 template <int NW, int MODE>
 __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsigned char *lds, int j0, int j1,
                                             float *__restrict__ part) {
@@ -90,7 +181,7 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
     const int l32 = lane & 31, hh = lane >> 5;
 
     if (q_len == 1 && !a.single) return;  // streamed by the decode launch
-    if (ctx < q_len) {                    // padding sequence: zero rows, no keys
+    if (ctx < q_len) {                          // padding sequence: zero rows, no keys
         const int row = r0 + l32;
         if (row < q_len) {
             bf16_t *o = a.out + ((long)(q_beg + row) * nq + head) * HD + hh * 64;
@@ -127,18 +218,51 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
 
     // ---- bf16 pages: DMA of the K/V tile of iteration `it` into (Kd, Vd): wave instruction i covers rows
     //      4*(wave + NW*i) .. +3; lane writes row + lane/16, physical chunk lane%16, so it reads the logical chunk that
-    //      swizzles onto it ----
+    //      swizzles onto it.
+    //
+    // Pages are looked up ahead of use, by vector loads: a scalar load in flight makes every wait for an LDS read a wait
+    // for all of them and for itself (both count on lgkmcnt), which cost 20 % of the time.  Where a wave needs one page
+    // a tile (BLOCK) or a DMA instruction (ROW4), lane l looks up entry l % LOOKS of tile l / LOOKS of the next PER
+    // tiles, PER tiles ahead, and the pages are read out as scalars; else each lane looks its own rows' pages up, a
+    // tile ahead. ----
     const int drow = lane >> 4, dchunk = lane & 15;
+    constexpr int RUN_ROWS = NW == 2 ? 2 : 1;  // 4-bit pages: rows of a tile whose runs a thread takes
+    constexpr bool BY_LANE = MODE == DMA_BLOCK || MODE == DMA_ROW4;
+    constexpr int LOOKS = MODE == KV4 ? RUN_ROWS : MODE == DMA_BLOCK ? 1 : LOADS, PER = BY_LANE ? 64 / LOOKS : 1;
+    int blk[BY_LANE ? 2 : LOOKS];  // BY_LANE: this lane's page of the current tiles and of the next ones
+    auto page_of = [&](int t) { return bs_shift >= 0 ? t >> bs_shift : t / block_size; };
+    auto lookup = [&](int it) {
+        if (it >= n_iter) return;
+        if constexpr (BY_LANE) {
+            const int at = min(it + lane / LOOKS, n_iter - 1);
+            const int kb0 = tile_key(at), last = kend - 1 - kb0;
+            const int r = MODE == DMA_BLOCK ? 0 : seen_row(4 * (wave + NW * (lane % LOOKS)), kb0, kt.lo, sinks, last);
+            blk[1] = bt[page_of(kb0 + r)];
+        } else {
+            const int kb0 = tile_key(it), last = kend - 1 - kb0;
+#pragma unroll
+            for (int i = 0; i < LOOKS; ++i) {
+                const int r = MODE == KV4 ? (tid & 255) / 4 + 32 * i : 4 * (wave + NW * i) + drow;
+                blk[i] = bt[page_of(kb0 + seen_row(r, kb0, kt.lo, sinks, last))];
+            }
+        }
+    };
+    auto page = [&](int it, int i) {
+        return BY_LANE ? __builtin_amdgcn_readlane(blk[0], it % PER * LOOKS + i) : blk[i % LOOKS];
+    };
     auto issue = [&](int it, bf16_t *Kd, bf16_t *Vd) {
         const bf16_t *kc = static_cast<const bf16_t *>(a.kc), *vc = static_cast<const bf16_t *>(a.vc);
         const long blk_stride = (long)nkv * block_size * HD;
         const long head_off = (long)kvh * block_size * HD;
         const int kb0 = tile_key(it);
         const int last = kend - 1 - kb0;
+        if (BY_LANE && it % PER == 0) {
+            blk[0] = blk[1];
+            lookup(it + PER);
+        }
         __amdgpu_buffer_rsrc_t krs, vrs;
         if (MODE == DMA_BLOCK) {  // the whole tile lies in one block: one descriptor pair per tile
-            const int phys = bt[__builtin_amdgcn_readfirstlane(kb0 >> bs_shift)];
-            const long base = (long)phys * blk_stride + head_off + (long)(kb0 & (block_size - 1)) * HD;
+            const long base = (long)page(it, 0) * blk_stride + head_off + (long)(kb0 & (block_size - 1)) * HD;
             krs = make_rsrc(kc + base, TILE * 2);
             vrs = make_rsrc(vc + base, TILE * 2);
         }
@@ -154,56 +278,67 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
             } else if (MODE == DMA_ROW4) {
                 const int first = seen_row(rbase, kb0, kt.lo, sinks, last);
                 const int t0 = __builtin_amdgcn_readfirstlane(kb0 + first);
-                const int bi = bs_shift >= 0 ? (t0 >> bs_shift) : t0 / block_size;
-                const long base = (long)bt[bi] * blk_stride + head_off + (long)(t0 - bi * block_size) * HD;
+                const long base =
+                    (long)page(it, i) * blk_stride + head_off + (long)(t0 - page_of(t0) * block_size) * HD;
                 const int voff = (src - first) * (HD * 2);
                 bufdma16(make_rsrc(kc + base, 4 * HD * 2), voff + kswz, Kd + rbase * HD);
                 bufdma16(make_rsrc(vc + base, 4 * HD * 2), voff + vswz, Vd + rbase * HD);
             } else {
                 const int t = kb0 + src;
-                const int bi = t / block_size;
-                const long at = (long)bt[bi] * blk_stride + head_off + (long)(t - bi * block_size) * HD;
+                const long at = (long)page(it, i) * blk_stride + head_off + (long)(t - page_of(t) * block_size) * HD;
                 dma16(kc + at + (kswz >> 1), Kd + rbase * HD);
                 dma16(vc + at + (vswz >> 1), Vd + rbase * HD);
             }
         }
+        if (!BY_LANE) lookup(it + 1);
     };
 
-    // ---- 4-bit pages: a tile is 64 rows x 4 runs of 32 values (16 bytes of codes and a scale byte) of K, then of V;
-    //      thread i takes runs i, i + 64 NW, ...  fetch() loads them into registers, commit() converts them into a stage
-    constexpr int RUNS = MODE == KV4 ? 8 / NW : 1;
-    u32x4_t run_codes[RUNS];
-    uint32_t run_scale[RUNS];
+    // ---- 4-bit pages: a tile is 64 rows x 4 runs of 32 values (16 bytes of codes and a scale byte) of K and of V.  A
+    //      thread takes run tid % 4 of row (tid % 256) / 4 (and of the row 32 further with 128 threads), of both K and V,
+    //      or with 512 threads of one of them.  fetch() loads runs into registers, commit() converts them into a stage
+    constexpr int RUN_KV = NW == 8 ? 1 : 2;
+    u32x4_t run_codes[RUN_ROWS][RUN_KV];
+    uint32_t run_scale[RUN_ROWS][RUN_KV];
     auto fetch = [&](int it) {
-        const int kb0 = tile_key(it), last = kend - 1 - kb0;
+        const int kb0 = tile_key(it), last = kend - 1 - kb0, run = tid & 3;
         const long hb = llmgen_cache::head_bytes(block_size);
 #pragma unroll
-        for (int i = 0; i < RUNS; ++i) {
-            const int c = tid + i * 64 * NW, r = (c & 255) >> 2, run = c & 3;
-            const int t = kb0 + seen_row(r, kb0, kt.lo, sinks, last);
-            const int bi = bs_shift >= 0 ? t >> bs_shift : t / block_size;
-            const int off = t - bi * block_size;
-            const uint8_t *p = static_cast<const uint8_t *>(c < 256 ? a.kc : a.vc) + ((long)bt[bi] * nkv + kvh) * hb;
-            run_codes[i] = ld16(p + (long)off * llmgen_cache::CODE_BYTES + run * 16);
-            run_scale[i] = p[(long)block_size * llmgen_cache::CODE_BYTES + (long)off * llmgen_cache::SCALE_BYTES + run];
+        for (int i = 0; i < (MODE == KV4 ? RUN_ROWS : 0); ++i) {
+            const int t = kb0 + seen_row((tid & 255) / 4 + 32 * i, kb0, kt.lo, sinks, last);
+            const int off = t - page_of(t) * block_size;
+            const long at = ((long)page(it, i) * nkv + kvh) * hb;
+#pragma unroll
+            for (int j = 0; j < RUN_KV; ++j) {
+                const uint8_t *p = static_cast<const uint8_t *>((RUN_KV == 1 ? tid >= 256 : j) ? a.vc : a.kc) + at;
+                run_codes[i][j] = ld16(p + (long)off * llmgen_cache::CODE_BYTES + run * 16);
+                run_scale[i][j] =
+                    p[(long)block_size * llmgen_cache::CODE_BYTES + (long)off * llmgen_cache::SCALE_BYTES + run];
+            }
         }
+        lookup(it + 1);
     };
     auto commit = [&](bf16_t *Kd, bf16_t *Vd) {
 #pragma unroll
-        for (int i = 0; i < RUNS; ++i) {
-            const int c = tid + i * 64 * NW, r = (c & 255) >> 2, run = c & 3;
-            const float sc = llmgen_cache::kv4_scale(run_scale[i]);
+        for (int i = 0; i < RUN_ROWS; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                bf16_t *dst = c < 256 ? Kd + k_off(r, run * 4 + j) : Vd + v_off(r, run * 4 + j);
-                *reinterpret_cast<u32x4_t *>(dst) = llmgen_cache::kv4_to_bf16(run_codes[i][j], sc);
+            for (int j = 0; j < RUN_KV; ++j) {
+                const int r = (tid & 255) / 4 + 32 * i, run = tid & 3;
+                const bool is_v = RUN_KV == 1 ? tid >= 256 : j;
+                const float sc = llmgen_cache::kv4_scale(run_scale[i][j]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    bf16_t *dst = is_v ? Vd + v_off(r, run * 4 + c) : Kd + k_off(r, run * 4 + c);
+                    *reinterpret_cast<u32x4_t *>(dst) = llmgen_cache::kv4_to_bf16(run_codes[i][j][c], sc);
+                }
             }
-        }
     };
 
     f32x16_t o[4];
-    float m_run, l_run;
-    bool careful = false;  // the second run of a unit that met an infinity or NaN
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
 
     // per-lane LDS offsets of the V^T fragment reads (ds_read_b64_tr_b16): 16-lane group g4, lane i = 4j + m;
     // the fragment's k-slots (hh*8 + e) are keys kc16*16 + (e/4)*8 + hh*4 + e%4, so the two reads of a fragment
@@ -227,11 +362,6 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
     // One 64-key tile for this wave: S^T = K Q^T, online softmax (base 2, scale folded into one FMA), O^T += V^T P^T.
     auto tile_step = [&](int kb0, const bf16_t *Ks, const bf16_t *Vs, auto masked) {
         constexpr bool MASK = decltype(masked)::value;
-        // offset `off` of this lane's keys (key kb0 + off + hh*4) is hidden from its row when it lies past the row's
-        // position (or the row is padding), or before its window and behind the sinks
-        const int lim = row_valid ? my_pos - kb0 - hh * 4 : -1;
-        const int lim_lo = my_pos - window - kb0 - hh * 4, lim_s = sinks - kb0 - hh * 4;
-        auto hidden = [&](int off) { return off > lim || (off <= lim_lo && off >= lim_s); };
         f32x16_t sacc[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -267,11 +397,24 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
         __builtin_amdgcn_sched_barrier(0);
         // lane holds row my_row, keys kb0 + kb*32 + (r/4)*8 + hh*4 + r%4 (raw dot products)
         if (MASK) {
+            // Key kb0 + off + hh*4 is hidden from the row when it lies past its position (or the row is padding), or
+            // before its window and behind the sinks: one bit an offset, then two instructions a score (the bit spread
+            // over a word, and a bitwise select of -inf)
+            auto above = [](int x) -> uint64_t {  // bits of the offsets > x
+                return x < 0 ? ~0ull : x >= 63 ? 0ull : ~0ull << (x + 1);
+            };
+            const int at = kb0 + hh * 4;
+            const uint64_t hid =
+                above(row_valid ? my_pos - at : -1) | (~above(my_pos - window - at) & above(sinks - at - 1));
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (hidden(kb * 32 + (r >> 2) * 8 + (r & 3))) sacc[kb][r] = -INFINITY;
+                for (int r = 0; r < 16; ++r) {
+                    const uint32_t bits = (uint32_t)(hid >> (32 * kb));
+                    const uint32_t m = (uint32_t)((int)(bits << (31 - ((r >> 2) * 8 + (r & 3)))) >> 31);
+                    const float x = sacc[kb][r];
+                    sacc[kb][r] = __builtin_bit_cast(float, (m & 0xff800000u) | (~m & __builtin_bit_cast(uint32_t, x)));
+                }
         }
         auto row_max = [&]() {
             float mx = -INFINITY;
@@ -330,57 +473,6 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[db][r] *= corr;
         }
-        if constexpr (MASK) {
-            if (careful) {
-                typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
-                bf16x8_t see[4];  // 1 for this lane's keys that its row sees, laid out as the probabilities are
-#pragma unroll
-                for (int kc16 = 0; kc16 < 4; ++kc16)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int r = (kc16 & 1) * 8 + e;
-                        see[kc16][e] = (__bf16)(hidden((kc16 >> 1) * 32 + (r >> 2) * 8 + (r & 3)) ? 0.f : 1.f);
-                    }
-#pragma unroll
-                for (int db = 0; db < 4; ++db) {
-                    // the finite values, and how many visible keys hold +inf, -inf and NaN in each place
-                    f32x16_t count[3];
-#pragma unroll
-                    for (int w = 0; w < 3; ++w)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) count[w][r] = 0.f;
-#pragma unroll
-                    for (int kc16 = 0; kc16 < 4; ++kc16) {
-                        vread(kc16 * 4 + db);
-                        const u16x8_t v = __builtin_bit_cast(u16x8_t, va[kc16 * 4 + db]);
-                        u16x8_t f = v;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if ((v[e] & 0x7f80u) == 0x7f80u) f[e] = 0;
-                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, f), pf[kc16], o[db],
-                                                                        0, 0, 0);
-#pragma unroll
-                        for (int w = 0; w < 3; ++w) {
-                            u16x8_t is;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const bool hit = w == 0 ? v[e] == 0x7f80u : w == 1 ? v[e] == 0xff80u : (v[e] & 0x7fffu) > 0x7f80u;
-                                is[e] = hit ? 0x3f80u : 0;  // 1 or 0
-                            }
-                            count[w] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, is), see[kc16],
-                                                                               count[w], 0, 0, 0);
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        if (count[0][r] > 0.f) o[db][r] += INFINITY;
-                        if (count[1][r] > 0.f) o[db][r] -= INFINITY;
-                        if (count[2][r] > 0.f) o[db][r] = NAN;
-                    }
-                }
-                return;
-            }
-        }
         // ---- O^T[dim][row] += V^T P^T: four independent accumulators per 16-key step ----
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -400,93 +492,110 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
             tile_step(kb0, Ks, Vs, std::false_type{});
     };
 
-    for (int run = 0;; ++run) {
+    lookup(0);
+    if constexpr (MODE == KV4) {
+        // The runs of tile it + 1 were fetched a tile ago; they are converted into the other stage beside the products of
+        // tile it.  Waves 4-7 share a SIMD each with waves 0-3 and convert behind their products, the others before
+        // them, so that one wave's conversions run beside the other's products.
+        const bool early = __builtin_amdgcn_readfirstlane(wave) < 4;
+        auto turn = [&](int it, const bf16_t *Ks, const bf16_t *Vs, bf16_t *Kn, bf16_t *Vn) {
+            auto next = [&]() {
+                if (it + 1 < n_iter) commit(Kn, Vn);
+                if (it + 2 < n_iter) fetch(it + 2);
+            };
+            if (NW < 8 || early) next();
+            compute(it, Ks, Vs);
+            if (NW == 8 && !early) next();
+            __syncthreads();
+        };
+        fetch(0);
+        commit(K0, V0);
+        if (!ONE_STAGE && n_iter > 1) fetch(1);
+        __syncthreads();
+        if constexpr (ONE_STAGE) {
+            for (int it = 0; it < n_iter; ++it) {
+                if (it + 1 < n_iter) fetch(it + 1);
+                compute(it, K0, V0);
+                __syncthreads();  // every wave is done reading the tile
+                if (it + 1 < n_iter) commit(K0, V0);
+                __syncthreads();
+            }
+        } else {
+            for (int it = 0; it < n_iter; it += 2) {
+                turn(it, K0, V0, K1, V1);
+                if (it + 1 >= n_iter) break;
+                turn(it + 1, K1, V1, K0, V0);
+            }
+        }
+    } else if constexpr (ONE_STAGE) {
+        for (int it = 0; it < n_iter; ++it) {
+            issue(it, K0, V0);
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();  // the tile has landed for every wave
+            compute(it, K0, V0);
+            __syncthreads();  // every wave is done reading it
+        }
+    } else {
+        // two LDS stages; the loop is unrolled twice so every DMA targets a fixed buffer (the compiler can then see
+        // that the reads of one stage never wait for the DMA into the other)
+        issue(0, K0, V0);
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        for (int it = 0; it < n_iter; it += 2) {
+            if (it + 1 < n_iter) issue(it + 1, K1, V1);
+            compute(it, K0, V0);
+            __builtin_amdgcn_s_waitcnt(0);  // this wave's DMA into stage 1 has landed
+            __syncthreads();                // ... and everyone's; everyone is done reading stage 0
+            if (it + 1 >= n_iter) break;
+            if (it + 2 < n_iter) issue(it + 2, K0, V0);
+            compute(it + 1, K1, V1);
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+        }
+    }
+    if (!wave_active) return;
+    const float l_tot = l_run + lane_xor(l_run, 32);
+    uint64_t again;  // rows to compute again (bits 0-31)
+    {
+        float z = 0.f;  // stays 0 unless an accumulator is an infinity or NaN
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
-        m_run = -INFINITY;
-        l_run = 0.f;
-        if constexpr (MODE == KV4) {
-            fetch(0);
-            for (int it = 0; it < n_iter; it += 2) {
-                commit(K0, V0);
-                __syncthreads();  // the tile is there, and everyone is done with the stage written next
-                if (it + 1 < n_iter) fetch(it + 1);
-                compute(it, K0, V0);
-                if (ONE_STAGE) __syncthreads();
-                if (it + 1 >= n_iter) break;
-                commit(K1, V1);
-                __syncthreads();
-                if (it + 2 < n_iter) fetch(it + 2);
-                compute(it + 1, K1, V1);
-                if (ONE_STAGE) __syncthreads();
-            }
-        } else if constexpr (ONE_STAGE) {
-            for (int it = 0; it < n_iter; ++it) {
-                issue(it, K0, V0);
-                __builtin_amdgcn_s_waitcnt(0);
-                __syncthreads();  // the tile has landed for every wave
-                compute(it, K0, V0);
-                __syncthreads();  // every wave is done reading it
-            }
-        } else {
-            // two LDS stages; the loop is unrolled twice so every DMA targets a fixed buffer (the compiler can then see
-            // that the reads of one stage never wait for the DMA into the other)
-            issue(0, K0, V0);
-            __builtin_amdgcn_s_waitcnt(0);
-            __syncthreads();
-            for (int it = 0; it < n_iter; it += 2) {
-                if (it + 1 < n_iter) issue(it + 1, K1, V1);
-                compute(it, K0, V0);
-                __builtin_amdgcn_s_waitcnt(0);  // this wave's DMA into stage 1 has landed
-                __syncthreads();                // ... and everyone's; everyone is done reading stage 0
-                if (it + 1 >= n_iter) break;
-                if (it + 2 < n_iter) issue(it + 2, K0, V0);
-                compute(it + 1, K1, V1);
-                __builtin_amdgcn_s_waitcnt(0);
-                __syncthreads();
-            }
-        }
-        if (run == 1) break;
-        float z = 0.f;  // stays 0 unless an accumulator of a row of the segment is an infinity or NaN
-        if (wave_active && row_valid) {
+            for (int r = 0; r < 16; ++r) z = __builtin_fmaf(o[db][r], 0.f, z);
+        again = __ballot(row_valid && !(z == 0.f) && l_tot == l_tot);
+        again = (again | again >> 32) & 0xffffffffu;
+    }
+    const bool mine = row_valid && !(again >> l32 & 1);
+
+    if (part) {  // leave the partial result (the merging workgroup reads it with device-coherent loads)
+        float *pw = part + wave * PART_WAVE_FLOATS + lane;
+        if (mine || !row_valid) {
 #pragma unroll
             for (int db = 0; db < 4; ++db)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) z = __builtin_fmaf(o[db][r], 0.f, z);
+                for (int r = 0; r < 16; ++r)
+                    __hip_atomic_store(pw + (db * 16 + r) * 64, o[db][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(pw + 64 * 64, m_run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(pw + 65 * 64, l_run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        if (!__syncthreads_or(!(z == 0.f))) break;
-        careful = true;
-    }
-
-    if (part) {  // leave the partial result (the merging workgroup reads it with device-coherent loads)
-        if (!wave_active) return;
-        float *pw = part + wave * PART_WAVE_FLOATS + lane;
+    } else if (mine) {  // normalise and store: lane holds dims db*32 + (r/4)*8 + hh*4 + r%4 of row my_row
+        const float inv = 1.f / l_tot;
+        bf16_t *orow = a.out + ((long)(q_beg + my_row) * nq + head) * HD + hh * 4;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                __hip_atomic_store(pw + (db * 16 + r) * 64, o[db][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(pw + 64 * 64, m_run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(pw + 65 * 64, l_run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        return;
+            for (int rr = 0; rr < 4; ++rr) {
+                u32x2_t w;
+                w[0] = pack_bf16x2(o[db][rr * 4 + 0] * inv, o[db][rr * 4 + 1] * inv);
+                w[1] = pack_bf16x2(o[db][rr * 4 + 2] * inv, o[db][rr * 4 + 3] * inv);
+                *reinterpret_cast<u32x2_t *>(orow + db * 32 + rr * 8) = w;
+            }
     }
-    // ---- normalise and store: lane holds dims db*32 + (r/4)*8 + hh*4 + r%4 of row my_row ----
-    if (!wave_active) return;
-    const float l_tot = l_run + lane_xor(l_run, 32);
-    if (!row_valid) return;
-    const float inv = 1.f / l_tot;
-    bf16_t *orow = a.out + ((long)(q_beg + my_row) * nq + head) * HD + hh * 4;
-#pragma unroll
-    for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int rr = 0; rr < 4; ++rr) {
-            u32x2_t w;
-            w[0] = pack_bf16x2(o[db][rr * 4 + 0] * inv, o[db][rr * 4 + 1] * inv);
-            w[1] = pack_bf16x2(o[db][rr * 4 + 2] * inv, o[db][rr * 4 + 3] * inv);
-            *reinterpret_cast<u32x2_t *>(orow + db * 32 + rr * 8) = w;
-        }
+    for (; again; again &= again - 1) {
+        const int r = __builtin_ctzll(again);
+        redo_row<MODE>(a, bt, kvh, ((long)(q_beg + r0 + r) * nq + head) * HD, base_pos + r0 + r, kt, j0, n_iter,
+                       part ? part + wave * PART_WAVE_FLOATS : nullptr, r);
+    }
 }
 
 }  // namespace llmgen_window
