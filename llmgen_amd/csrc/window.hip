@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)
     if (NW <= 4 && P > 1) {  // which share of the unit's key tiles
         const int tile = a.n_tiles - 1 - unit / (a.nkv * a.head_groups);
         const int s = a.tile_seq[tile], q0 = a.tile_q0[tile], q_len = a.cu_q[s + 1] - a.cu_q[s];
-        const int ctx = (int)min((long)a.ctx_lens[s], (long)a.max_blocks * a.block_size);
+        const int ctx = (int)min((long)a.ctx_lens[s], (long)a.max_blocks * a.div.bs);
         const int n = (q_len > 1 || a.single) && ctx >= q_len
                           ? key_tiles(ctx - q_len + q0, ctx - q_len + min(q0 + BQ, q_len), a.window, a.sinks).n
                           : 0;
@@ -194,7 +194,7 @@ void prefill(const char *who, bool kv4, bf16_t *out, const bf16_t *q, const void
         }
     }
     const WindowArgs a{out, q, kc, vc, bt, ctx, cu_q, tile_seq, tile_q0, n_tiles, nq, nkv, G, G / (nw / 2), max_blocks,
-                       block_size, bs_shift, sl2, window, sinks, single_rows == 0};
+                       llmgen_cache::page_div(block_size), sl2, window, sinks, single_rows == 0};
     if (nw == 2) launch_prefill<2>(mode, a, units, (int)P, w);
     else if (nw == 4) launch_prefill<4>(mode, a, units, (int)P, w);
     else launch_prefill<8>(mode, a, units, 1, w);

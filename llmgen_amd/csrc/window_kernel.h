@@ -42,6 +42,24 @@ __device__ __forceinline__ int seen_row(int r, int kb0, int lo, int sinks, int l
     return min(x, last);
 }
 
+// bufdma16 with a wave-uniform byte offset of its own
+__device__ __forceinline__ void bufdma16s(__amdgpu_buffer_rsrc_t rs, int voff, int soff, bf16_t *ldst) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)ldst, 16, voff, soff, 0, 0);
+}
+
+// Element offset of (row, 16-byte chunk) in a K or V tile.  Tiles that DMA fills have the layouts of prefill_kernel.h;
+// those of 4-bit pages are written by lanes (rows r, r + 4, r + 8, r + 12 and all 16 chunks in any 16 consecutive lanes),
+// and this swizzle spreads these writes over all banks as well as both kinds of fragment reads.
+template <int MODE>
+__device__ __forceinline__ int k_place(int row, int chunk) {
+    if (MODE != KV4) return k_off(row, chunk);
+    return row * HD + ((chunk ^ ((row & 3) << 2 | (row >> 2 & 3))) << 3);
+}
+template <int MODE>
+__device__ __forceinline__ int v_place(int row, int chunk) {
+    return MODE != KV4 ? v_off(row, chunk) : k_place<KV4>(row, chunk);
+}
+
 template <int NW>
 struct WindowLds {
     // two stages of one 64-key K and V tile; 2-wave workgroups keep one, so that four share a CU
@@ -57,7 +75,8 @@ struct WindowArgs {
     const bf16_t *q;
     const void *kc, *vc;
     const int *block_tables, *ctx_lens, *cu_q, *tile_seq, *tile_q0;
-    int n_tiles, nq, nkv, G, head_groups, max_blocks, block_size, bs_shift;
+    int n_tiles, nq, nkv, G, head_groups, max_blocks;
+    llmgen_cache::PageDiv div;
     float scale_log2;
     int window, sinks;
     bool single;  // segments of one row are computed here (no decode launch for them)
@@ -70,10 +89,10 @@ template <int MODE>
 __device__ __forceinline__ void redo_row(const WindowArgs &a, const int *bt, int kvh, long row, int pos, const KeyTiles &kt,
                                          int j0, int n, float *part, int r) {
     const int lane = threadIdx.x & 63;
-    const long hb = MODE == KV4 ? llmgen_cache::head_bytes(a.block_size) : (long)a.block_size * HD * 2;
+    const long hb = MODE == KV4 ? llmgen_cache::head_bytes(a.div.bs) : (long)a.div.bs * HD * 2;
     auto place = [&](int t, int &off) {  // key t's page and head, and its row there
-        const int blk = t / a.block_size;
-        off = t - blk * a.block_size;
+        const int blk = a.div(t);
+        off = t - blk * a.div.bs;
         return ((long)bt[blk] * a.nkv + kvh) * hb;
     };
     float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
@@ -92,7 +111,7 @@ __device__ __forceinline__ void redo_row(const WindowArgs &a, const int *bt, int
                 float sc = 0.f;
                 if (MODE == KV4) {
                     codes = ld16(p + (long)off * llmgen_cache::CODE_BYTES + run * 16);
-                    sc = llmgen_cache::kv4_scale(p[(long)a.block_size * llmgen_cache::CODE_BYTES +
+                    sc = llmgen_cache::kv4_scale(p[(long)a.div.bs * llmgen_cache::CODE_BYTES +
                                                    (long)off * llmgen_cache::SCALE_BYTES + run]);
                 }
 #pragma unroll
@@ -128,7 +147,7 @@ __device__ __forceinline__ void redo_row(const WindowArgs &a, const int *bt, int
             if (MODE == KV4) {
                 const uint32_t code = v[(long)off * llmgen_cache::CODE_BYTES + lane];
                 w = llmgen_cache::kv4_to_bf16(code, llmgen_cache::kv4_scale(
-                    v[(long)a.block_size * llmgen_cache::CODE_BYTES + (long)off * llmgen_cache::SCALE_BYTES + lane / 16]))[0];
+                    v[(long)a.div.bs * llmgen_cache::CODE_BYTES + (long)off * llmgen_cache::SCALE_BYTES + lane / 16]))[0];
             } else {
                 w = *reinterpret_cast<const uint32_t *>(v + (long)off * (HD * 2) + lane * 4);
             }
@@ -165,7 +184,7 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
     constexpr bool ONE_STAGE = WindowLds<NW>::ONE_STAGE;
     bf16_t *K0 = sm.K0, *V0 = sm.V0, *K1 = ONE_STAGE ? sm.K0 : sm.K1, *V1 = ONE_STAGE ? sm.V0 : sm.V1;
 
-    const int nq = a.nq, nkv = a.nkv, block_size = a.block_size, bs_shift = a.bs_shift;
+    const int nq = a.nq, nkv = a.nkv, block_size = a.div.bs;
     const int window = a.window, sinks = a.sinks;
     const float scale_log2 = a.scale_log2;
     const int kvh = bid % nkv;
@@ -226,30 +245,41 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
     // tiles, PER tiles ahead, and the pages are read out as scalars; else each lane looks its own rows' pages up, a
     // tile ahead. ----
     const int drow = lane >> 4, dchunk = lane & 15;
-    constexpr int RUN_ROWS = NW == 2 ? 2 : 1;  // 4-bit pages: rows of a tile whose runs a thread takes
+    // 4-bit pages: rows of a tile whose runs a thread takes (4 consecutive threads share a row, 16 take rows 4 apart)
+    constexpr int RUN_ROWS = NW == 2 ? 2 : 1;
+    const int run4 = (tid & 255) >> 2, my_run_row = (run4 & ~15) | (run4 & 3) << 2 | (run4 >> 2 & 3);
+    const long hb = llmgen_cache::head_bytes(block_size);
     constexpr bool BY_LANE = MODE == DMA_BLOCK || MODE == DMA_ROW4;
     constexpr int LOOKS = MODE == KV4 ? RUN_ROWS : MODE == DMA_BLOCK ? 1 : LOADS, PER = BY_LANE ? 64 / LOOKS : 1;
     int blk[BY_LANE ? 2 : LOOKS];  // BY_LANE: this lane's page of the current tiles and of the next ones
-    auto page_of = [&](int t) { return bs_shift >= 0 ? t >> bs_shift : t / block_size; };
     auto lookup = [&](int it) {
         if (it >= n_iter) return;
         if constexpr (BY_LANE) {
             const int at = min(it + lane / LOOKS, n_iter - 1);
             const int kb0 = tile_key(at), last = kend - 1 - kb0;
             const int r = MODE == DMA_BLOCK ? 0 : seen_row(4 * (wave + NW * (lane % LOOKS)), kb0, kt.lo, sinks, last);
-            blk[1] = bt[page_of(kb0 + r)];
+            blk[1] = bt[a.div(kb0 + r)];
         } else {
             const int kb0 = tile_key(it), last = kend - 1 - kb0;
 #pragma unroll
             for (int i = 0; i < LOOKS; ++i) {
-                const int r = MODE == KV4 ? (tid & 255) / 4 + 32 * i : 4 * (wave + NW * i) + drow;
-                blk[i] = bt[page_of(kb0 + seen_row(r, kb0, kt.lo, sinks, last))];
+                const int r = MODE == KV4 ? my_run_row + 32 * i : 4 * (wave + NW * i) + drow;
+                blk[i] = bt[a.div(kb0 + seen_row(r, kb0, kt.lo, sinks, last))];
             }
         }
     };
     auto page = [&](int it, int i) {
         return BY_LANE ? __builtin_amdgcn_readlane(blk[0], it % PER * LOOKS + i) : blk[i % LOOKS];
     };
+    constexpr int KSWZ = NW == 2 ? 2 : 1;
+    int k_lane[KSWZ], v_lane;
+    {
+        const int first = MODE == DMA_BLOCK ? 4 * wave + drow : drow;  // from the descriptor's row
+#pragma unroll
+        for (int i = 0; i < KSWZ; ++i)
+            k_lane[i] = first * (HD * 2) + ((dchunk ^ ((4 * (wave + NW * i) + drow) & 15)) << 4);
+        v_lane = first * (HD * 2) + ((dchunk ^ ((drow << 2) & 15)) << 4);
+    }
     auto issue = [&](int it, bf16_t *Kd, bf16_t *Vd) {
         const bf16_t *kc = static_cast<const bf16_t *>(a.kc), *vc = static_cast<const bf16_t *>(a.vc);
         const long blk_stride = (long)nkv * block_size * HD;
@@ -266,6 +296,25 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
             krs = make_rsrc(kc + base, TILE * 2);
             vrs = make_rsrc(vc + base, TILE * 2);
         }
+        if (BY_LANE && (kb0 >= kt.lo || kb0 + BK <= sinks) && last >= BK - 1) {
+            // every row of the tile is read: the lanes' offsets are the same in each such tile.  They repeat from one
+            // instruction to the next (every second one where 4 NW rows are half a swizzle period)
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int rbase = 4 * (wave + NW * i), soff = NW * 4 * (HD * 2) * i;
+                if (MODE == DMA_BLOCK) {
+                    bufdma16s(krs, k_lane[i % KSWZ], soff, Kd + rbase * HD);
+                    bufdma16s(vrs, v_lane, soff, Vd + rbase * HD);
+                } else {
+                    const int t0 = __builtin_amdgcn_readfirstlane(kb0 + rbase);
+                    const long base =
+                        (long)page(it, i) * blk_stride + head_off + (long)(t0 - a.div(t0) * block_size) * HD;
+                    bufdma16(make_rsrc(kc + base, 4 * HD * 2), k_lane[i % KSWZ], Kd + rbase * HD);
+                    bufdma16(make_rsrc(vc + base, 4 * HD * 2), v_lane, Vd + rbase * HD);
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int rbase = 4 * (wave + NW * i);
@@ -279,13 +328,13 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
                 const int first = seen_row(rbase, kb0, kt.lo, sinks, last);
                 const int t0 = __builtin_amdgcn_readfirstlane(kb0 + first);
                 const long base =
-                    (long)page(it, i) * blk_stride + head_off + (long)(t0 - page_of(t0) * block_size) * HD;
+                    (long)page(it, i) * blk_stride + head_off + (long)(t0 - a.div(t0) * block_size) * HD;
                 const int voff = (src - first) * (HD * 2);
                 bufdma16(make_rsrc(kc + base, 4 * HD * 2), voff + kswz, Kd + rbase * HD);
                 bufdma16(make_rsrc(vc + base, 4 * HD * 2), voff + vswz, Vd + rbase * HD);
             } else {
                 const int t = kb0 + src;
-                const long at = (long)page(it, i) * blk_stride + head_off + (long)(t - page_of(t) * block_size) * HD;
+                const long at = (long)page(it, i) * blk_stride + head_off + (long)(t - a.div(t) * block_size) * HD;
                 dma16(kc + at + (kswz >> 1), Kd + rbase * HD);
                 dma16(vc + at + (vswz >> 1), Vd + rbase * HD);
             }
@@ -294,25 +343,27 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
     };
 
     // ---- 4-bit pages: a tile is 64 rows x 4 runs of 32 values (16 bytes of codes and a scale byte) of K and of V.  A
-    //      thread takes run tid % 4 of row (tid % 256) / 4 (and of the row 32 further with 128 threads), of both K and V,
-    //      or with 512 threads of one of them.  fetch() loads runs into registers, commit() converts them into a stage
+    //      thread takes run tid % 4 of row my_run_row (and of the row 32 further with 128 threads), of both K and V, or
+    //      with 512 threads of one of them.  fetch() loads runs into registers, commit() converts them into a stage
     constexpr int RUN_KV = NW == 8 ? 1 : 2;
     u32x4_t run_codes[RUN_ROWS][RUN_KV];
     uint32_t run_scale[RUN_ROWS][RUN_KV];
     auto fetch = [&](int it) {
         const int kb0 = tile_key(it), last = kend - 1 - kb0, run = tid & 3;
-        const long hb = llmgen_cache::head_bytes(block_size);
+        const bool all = (kb0 >= kt.lo || kb0 + BK <= sinks) && last >= BK - 1;  // every row of the tile is read
 #pragma unroll
         for (int i = 0; i < (MODE == KV4 ? RUN_ROWS : 0); ++i) {
-            const int t = kb0 + seen_row((tid & 255) / 4 + 32 * i, kb0, kt.lo, sinks, last);
-            const int off = t - page_of(t) * block_size;
-            const long at = ((long)page(it, i) * nkv + kvh) * hb;
+            const int r = my_run_row + 32 * i;
+            const int t = kb0 + (all ? r : seen_row(r, kb0, kt.lo, sinks, last));
+            const int off = t - a.div(t) * block_size;
+            const long at = ((long)blk[i] * nkv + kvh) * hb;
+            const int codes = off * llmgen_cache::CODE_BYTES + run * 16;
+            const int scale = block_size * llmgen_cache::CODE_BYTES + off * llmgen_cache::SCALE_BYTES + run;
 #pragma unroll
             for (int j = 0; j < RUN_KV; ++j) {
                 const uint8_t *p = static_cast<const uint8_t *>((RUN_KV == 1 ? tid >= 256 : j) ? a.vc : a.kc) + at;
-                run_codes[i][j] = ld16(p + (long)off * llmgen_cache::CODE_BYTES + run * 16);
-                run_scale[i][j] =
-                    p[(long)block_size * llmgen_cache::CODE_BYTES + (long)off * llmgen_cache::SCALE_BYTES + run];
+                run_codes[i][j] = ld16(p + codes);
+                run_scale[i][j] = p[scale];
             }
         }
         lookup(it + 1);
@@ -322,14 +373,12 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
         for (int i = 0; i < RUN_ROWS; ++i)
 #pragma unroll
             for (int j = 0; j < RUN_KV; ++j) {
-                const int r = (tid & 255) / 4 + 32 * i, run = tid & 3;
-                const bool is_v = RUN_KV == 1 ? tid >= 256 : j;
+                bf16_t *dst = (RUN_KV == 1 ? tid >= 256 : j) ? Vd : Kd;
                 const float sc = llmgen_cache::kv4_scale(run_scale[i][j]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    bf16_t *dst = is_v ? Vd + v_off(r, run * 4 + c) : Kd + k_off(r, run * 4 + c);
-                    *reinterpret_cast<u32x4_t *>(dst) = llmgen_cache::kv4_to_bf16(run_codes[i][j][c], sc);
-                }
+                for (int c = 0; c < 4; ++c)
+                    *reinterpret_cast<u32x4_t *>(dst + k_place<KV4>(my_run_row + 32 * i, (tid & 3) * 4 + c)) =
+                        llmgen_cache::kv4_to_bf16(run_codes[i][j][c], sc);
             }
     };
 
@@ -343,25 +392,25 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
     // per-lane LDS offsets of the V^T fragment reads (ds_read_b64_tr_b16): 16-lane group g4, lane i = 4j + m;
     // the fragment's k-slots (hh*8 + e) are keys kc16*16 + (e/4)*8 + hh*4 + e%4, so the two reads of a fragment
     // take keys hh*4 + j (+8) and dims db*32 + (g4&1)*16 + 4m .. +3
-    int voff[4];
+    int voff[4], vhi[4];  // of keys j, and of keys 8 + j
     {
         const int g4 = lane >> 4, i = lane & 15, j = i >> 2, m = i & 3;
         const int key = (g4 >> 1) * 4 + j;
 #pragma unroll
         for (int db = 0; db < 4; ++db) {
             const int dim = db * 32 + (g4 & 1) * 16 + 4 * m;
-            voff[db] = v_off(key, dim >> 3) + (dim & 7);
+            voff[db] = v_place<MODE>(key, dim >> 3) + (dim & 7);
+            vhi[db] = v_place<MODE>(key + 8, dim >> 3) + (dim & 7);
         }
     }
     // per-lane LDS offsets of the K fragment reads (row l32, logical chunk 2c + hh); row 32 + l32 has the same
     // swizzle, so its offset is a constant 32 rows further
     int koff[8];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) koff[c] = k_off(l32, 2 * c + hh);
+    for (int c = 0; c < 8; ++c) koff[c] = k_place<MODE>(l32, 2 * c + hh);
 
     // One 64-key tile for this wave: S^T = K Q^T, online softmax (base 2, scale folded into one FMA), O^T += V^T P^T.
-    auto tile_step = [&](int kb0, const bf16_t *Ks, const bf16_t *Vs, auto masked) {
-        constexpr bool MASK = decltype(masked)::value;
+    auto tile_step = [&](int kb0, const bf16_t *Ks, const bf16_t *Vs, bool masked) {
         f32x16_t sacc[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -387,16 +436,16 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
         // depend on P and are read before the softmax
         bf16x8_t va[16];
         auto vread = [&](int i) {
-            const bf16_t *vp = Vs + (i >> 2) * 16 * HD + voff[i & 3];
-            const s16x4_t lo = ds_read_tr(vp);           // keys hh*4 + j
-            const s16x4_t hi = ds_read_tr(vp + 8 * HD);  // keys 8 + hh*4 + j
+            const bf16_t *vp = Vs + (i >> 2) * 16 * HD;
+            const s16x4_t lo = ds_read_tr(vp + voff[i & 3]);  // keys hh*4 + j
+            const s16x4_t hi = ds_read_tr(vp + vhi[i & 3]);   // keys 8 + hh*4 + j
             va[i] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         };
 #pragma unroll
         for (int i = 0; i < VPF; ++i) vread(i);
         __builtin_amdgcn_sched_barrier(0);
         // lane holds row my_row, keys kb0 + kb*32 + (r/4)*8 + hh*4 + r%4 (raw dot products)
-        if (MASK) {
+        if (masked) {
             // Key kb0 + off + hh*4 is hidden from the row when it lies past its position (or the row is padding), or
             // before its window and behind the sinks: one bit an offset, then two instructions a score (the bit spread
             // over a word, and a bitwise select of -inf)
@@ -485,11 +534,10 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
         const int kb0 = tile_key(it);
         if (!wave_active || kb0 > wave_pos_max) return;
         if (kb0 + BK - 1 <= wave_pos_min - window && kb0 >= sinks) return;  // before every row's window
-        // tiles that every row of the wave sees whole take the unmasked path
-        if (wave_has_pad || kb0 + BK - 1 > wave_pos_min || (kb0 <= wave_pos_max - window && kb0 + BK > sinks))
-            tile_step(kb0, Ks, Vs, std::true_type{});
-        else
-            tile_step(kb0, Ks, Vs, std::false_type{});
+        // One copy of the tile's code for masked and unmasked tiles (a branch around the masks): with two, the compiler
+        // keeps O in other registers in each and moves it between them, 60 instructions a tile.
+        tile_step(kb0, Ks, Vs, wave_has_pad || kb0 + BK - 1 > wave_pos_min ||
+                                   (kb0 <= wave_pos_max - window && kb0 + BK > sinks));
     };
 
     lookup(0);
