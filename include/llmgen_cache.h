@@ -102,7 +102,7 @@ void hip_attn_prefill_kv4(uint16_t *out, const uint16_t *q, const uint8_t *k_cac
  *
  * Copies page src[i] onto page dst[i] in each of n_pools pools (the K and V pools of every layer, of either kind of
  * page).  pools, src and dst are host arrays, read before the call returns: pools holds device pointers (16-byte
- * aligned), the pages are num_blocks x block_bytes (a multiple of 16).  Every id must lie in [0, num_blocks), no page
+ * aligned), the pages are num_blocks x block_bytes (a multiple of 16, at most 2^28).  Every id must lie in [0, num_blocks), no page
  * may be the destination of two pairs, and none both a source and a destination (src[i] == dst[i] is a pair that does
  * nothing): the pairs then have no order.  Otherwise nothing is copied.
  * ------------------------------------------------------------------------------------------------------- */

@@ -57,5 +57,5 @@ class BlockCopies:
         src, dst = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
         if src.shape != dst.shape or src.ndim != 1:
             raise ValueError("one destination for each source")
-        self._call(self._ptrs, len(self.pools), self.page_bytes, self.num_blocks, src.ctypes.data, dst.ctypes.data,
-                   src.size)
+        self._call(self._ptrs, len(self.pools), self.page_bytes, self.num_blocks, src.__array_interface__["data"][0],
+                   dst.__array_interface__["data"][0], src.size)

@@ -17,85 +17,110 @@ using namespace llmgen_cache;
 // ------------------------------------------------------------------------------------------------------------
 // HBM-bound copies with a conversion: 16 lanes take a row, 8 values (16 bytes of bf16, 4 bytes of codes) each, so a wave
 // moves 1 KB of bf16 in one access; the largest magnitude of a run of 32 is an integer maximum over the 4 lanes that
-// hold it (two DPP steps), and the conversion itself is the hardware's, two values an instruction.
-constexpr int ROW_LANES = 16, QUANT_THREADS = 256;
+// hold it (two DPP steps), and the conversion itself is the hardware's, two values an instruction.  Threads of large
+// calls take U = 4 rows, all loads issued before any conversion (16384 tokens x 8 heads,
+// 85 MB each: written in 20 us, read back in 15.5 us; with one row a thread 25 and 18 us).
+constexpr int ROW_LANES = 16, QUANT_THREADS = 256, ROWS_PER_PASS = QUANT_THREADS / ROW_LANES;
 
-// one step of a maximum over the quad
 template <int CTRL>
-__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
-    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false));
+__device__ __forceinline__ uint32_t dpp_u(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false);
 }
 
-// where row `row` = (token, kv head) of K or V goes: byte offset of its codes, and of its scales
-__device__ __forceinline__ void row_place(int slot, int h, int nkv, int block_size, long &codes, long &scales) {
-    const int blk = slot / block_size, off = slot - blk * block_size;
-    const long base = ((long)blk * nkv + h) * head_bytes(block_size);
-    codes = base + (long)off * CODE_BYTES;
-    scales = base + (long)block_size * CODE_BYTES + (long)off * SCALE_BYTES;
+// Row r of the call: K's rows (token, kv head), then V's.
+struct RowsArgs {
+    const int *slots;
+    int rows, nkv;
+    PageDiv per_token, per_page;  // division by nkv, and by the block size
+    long hb;
+};
+struct RowPlace {
+    bool in, live, is_v;  // a row of the call; one with a slot; of V
+    int row;              // within K or V
+    long codes, scales;  // byte offsets in the pool
+};
+__device__ __forceinline__ RowPlace row_place(const RowsArgs &a, int r) {
+    RowPlace p;
+    p.is_v = r >= a.rows;
+    p.row = p.is_v ? r - a.rows : r;
+    p.in = r < 2 * a.rows;
+    const int t = a.per_token(p.row), h = p.row - t * a.nkv;
+    const int slot = p.in ? a.slots[t] : -1;
+    p.live = slot >= 0;
+    const int blk = a.per_page(slot), off = slot - blk * a.per_page.bs;
+    const long base = ((long)blk * a.nkv + h) * a.hb;
+    p.codes = base + (long)off * CODE_BYTES;
+    p.scales = base + (long)a.per_page.bs * CODE_BYTES + (long)off * SCALE_BYTES;
+    return p;
 }
 
+template <int U>
 __global__ void __launch_bounds__(QUANT_THREADS) store_kv4_kernel(const bf16_t *__restrict__ k,
-                                                                  const bf16_t *__restrict__ v,
-                                                                  const int *__restrict__ slots,
-                                                                  uint8_t *__restrict__ kc, uint8_t *__restrict__ vc,
-                                                                  long rows, int nkv, int block_size) {
-    const long idx = (long)blockIdx.x * QUANT_THREADS + threadIdx.x;
-    const long r = idx / ROW_LANES;
-    const int c = (int)(idx % ROW_LANES);
-    if (r >= 2 * rows) return;  // whole rows leave together, so the quads below are full
-    const bool is_v = r >= rows;
-    const long row = is_v ? r - rows : r;
-    const int t = (int)(row / nkv), h = (int)(row - (long)t * nkv);
-    const int slot = slots[t];
-    if (slot < 0) return;
-    const u32x4_t x = ld16((is_v ? v : k) + row * HD + c * 8);
-    uint32_t top = 0;  // magnitude bits: they order as the values do, infinities and NaN above all
+                                                                  const bf16_t *__restrict__ v, uint8_t *__restrict__ kc,
+                                                                  uint8_t *__restrict__ vc, const RowsArgs a) {
+    const int c = threadIdx.x % ROW_LANES;
+    RowPlace p[U];
+    u32x4_t x[U];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
-    top = quad_max<0xB1>(top);
-    top = quad_max<0x4E>(top);
-    // floor(log2 amax) is the exponent field for normal numbers.  Subnormal ones have an amax below 2^-126, and e would
-    // fall below -127 for any amax under 2^-125: both take the clamp.  Mantissas above 1.75 (0x60 of 7 bits) round up.
-    const int field = (int)(top >> 7);
-    int byte = field - 2 + ((top & 0x7f) > 0x60 ? 1 : 0);
-    byte = top == 0 ? 0 : min(max(byte, 0), 252);
-    const bool bad = top >= 0x7f80u;
-    if (bad) byte = 255;
-    const float s = kv4_scale(bad ? 127 : byte);
-    const uint32_t x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];
-    uint32_t w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x0), s, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x1), s, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x2), s, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x3), s, 3);
-    if (bad) w = 0;
-    long codes, scales;
-    row_place(slot, h, nkv, block_size, codes, scales);
-    uint8_t *pool = is_v ? vc : kc;
-    *reinterpret_cast<uint32_t *>(pool + codes + c * 4) = w;
-    if ((c & 3) == 0) pool[scales + (c >> 2)] = (uint8_t)byte;
+    for (int u = 0; u < U; ++u) {
+        p[u] = row_place(a, ((int)blockIdx.x * U + u) * ROWS_PER_PASS + (int)(threadIdx.x / ROW_LANES));
+        // not held up by the slot; read once
+        if (p[u].in)
+            x[u] = __builtin_nontemporal_load(
+                reinterpret_cast<const u32x4_t *>((p[u].is_v ? v : k) + (long)p[u].row * HD + c * 8));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (!p[u].live) continue;  // a row's lanes leave together, so the quads below are full
+        const uint32_t x0 = x[u][0], x1 = x[u][1], x2 = x[u][2], x3 = x[u][3];
+        // magnitude bits: they order as the values do, infinities and NaN above all
+        uint32_t top = max(max(max(x0 & 0x7fffu, x0 >> 16 & 0x7fffu), max(x1 & 0x7fffu, x1 >> 16 & 0x7fffu)),
+                           max(max(x2 & 0x7fffu, x2 >> 16 & 0x7fffu), max(x3 & 0x7fffu, x3 >> 16 & 0x7fffu)));
+        top = max(top, dpp_u<0xB1>(top));
+        top = max(top, dpp_u<0x4E>(top));
+        // floor(log2 amax) is the exponent field for normal numbers.  Subnormal ones have an amax below 2^-126, and e
+        // would fall below -127 for any amax under 2^-125: both take the clamp.  Mantissas above 1.75 (0x60 of 7 bits)
+        // round up.
+        int byte = (int)(top >> 7) - 2 + ((top & 0x7f) > 0x60 ? 1 : 0);
+        byte = top == 0 ? 0 : min(max(byte, 0), 252);
+        const bool bad = top >= 0x7f80u;
+        if (bad) byte = 255;
+        const float s = kv4_scale(bad ? 127 : byte);
+        uint32_t w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x0), s, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x1), s, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x2), s, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x3), s, 3);
+        // the row's four scale bytes in one word: rotations by 4 and 8 lanes of the 16
+        uint32_t scales = (uint32_t)byte << (c >> 2) * 8;
+        scales |= dpp_u<0x124>(scales);
+        scales |= dpp_u<0x128>(scales);
+        uint8_t *pool = p[u].is_v ? vc : kc;
+        *reinterpret_cast<uint32_t *>(pool + p[u].codes + c * 4) = bad ? 0 : w;
+        if (c == 0) *reinterpret_cast<uint32_t *>(pool + p[u].scales) = scales;
+    }
 }
 
+template <int U>
 __global__ void __launch_bounds__(QUANT_THREADS) load_kv4_kernel(bf16_t *__restrict__ k, bf16_t *__restrict__ v,
-                                                                 const int *__restrict__ slots,
                                                                  const uint8_t *__restrict__ kc,
-                                                                 const uint8_t *__restrict__ vc, long rows, int nkv,
-                                                                 int block_size) {
-    const long idx = (long)blockIdx.x * QUANT_THREADS + threadIdx.x;
-    const long r = idx / ROW_LANES;
-    const int c = (int)(idx % ROW_LANES);
-    if (r >= 2 * rows) return;
-    const bool is_v = r >= rows;
-    const long row = is_v ? r - rows : r;
-    const int t = (int)(row / nkv), h = (int)(row - (long)t * nkv);
-    const int slot = slots[t];
-    if (slot < 0) return;
-    long codes, scales;
-    row_place(slot, h, nkv, block_size, codes, scales);
-    const uint8_t *pool = is_v ? vc : kc;
-    const uint32_t w = *reinterpret_cast<const uint32_t *>(pool + codes + c * 4);
-    const float s = kv4_scale(pool[scales + (c >> 2)]);
-    *reinterpret_cast<u32x4_t *>((is_v ? v : k) + row * HD + c * 8) = kv4_to_bf16(w, s);
+                                                                 const uint8_t *__restrict__ vc, const RowsArgs a) {
+    const int c = threadIdx.x % ROW_LANES;
+    RowPlace p[U];
+    uint32_t w[U], s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        p[u] = row_place(a, ((int)blockIdx.x * U + u) * ROWS_PER_PASS + (int)(threadIdx.x / ROW_LANES));
+        if (!p[u].live) continue;
+        const uint8_t *pool = p[u].is_v ? vc : kc;
+        w[u] = *reinterpret_cast<const uint32_t *>(pool + p[u].codes + c * 4);
+        s[u] = pool[p[u].scales + (c >> 2)];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (p[u].live)
+            *reinterpret_cast<u32x4_t *>((p[u].is_v ? v : k) + (long)p[u].row * HD + c * 8) =
+                kv4_to_bf16(w[u], kv4_scale(s[u]));
 }
 
 bool check_rows(const char *who, const void *k, const void *v, const void *slots, const void *kc, const void *vc, int T,
@@ -104,9 +129,17 @@ bool check_rows(const char *who, const void *k, const void *v, const void *slots
     if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc) & 15)
         return refuse(who, "tensors must be 16-byte aligned");
     if (hd != HD || nkv <= 0 || block_size <= 0) return refuse(who, "unsupported shape (head_dim must be 128)");
-    if ((long)T * nkv * 2 * ROW_LANES / QUANT_THREADS >= 0x7fffffffL) return refuse(who, "too many rows");
+    if ((long)T * nkv >= 1L << 30) return refuse(who, "too many rows");
     return true;
 }
+
+RowsArgs rows_args(const int *slots, int T, int nkv, int block_size) {
+    return RowsArgs{slots, T * nkv, nkv, page_div(nkv), page_div(block_size), head_bytes(block_size)};
+}
+// Workgroups for `rows` rows of K and of V at U rows a thread.
+unsigned row_groups(int rows, int U) { return (unsigned)((2L * rows + U * ROWS_PER_PASS - 1) / (U * ROWS_PER_PASS)); }
+// Four rows a thread once that still leaves four workgroups a CU.
+int rows_a_thread(int rows) { return row_groups(rows, 4) >= 4u * llmgen_num_cus() ? 4 : 1; }
 
 // ------------------------------------------------------------------------------------------------------------
 // Split-K decode
@@ -123,8 +156,9 @@ bool check_rows(const char *who, const void *k, const void *v, const void *slots
 //     probabilities, rounded to bf16 (half a step, 2^-9, as the other attention kernels), are the B fragment of
 //     O^T = V^T P^T as they stand: the fragment's k-slots are assigned to keys in the order the accumulator holds them.
 //   * V: lane l loads bytes 16 l of the tile (key l / 4, run l % 4), converts them and puts the bf16 row into the wave's
-//     8 KB of LDS, from where ds_read_b64_tr_b16 reads it transposed.  Chunks of 16 bytes are swizzled by the row
-//     (chunk ^ 2 (row & 7)) so that both directions spread over the banks.
+//     8 KB of LDS, from where ds_read_b64_tr_b16 reads it transposed.  Chunks of 16 bytes are swizzled by the row:
+//     writes put 4 rows at once into chunks that differ in bits 2 and 3 only, reads take a pair of chunks of 8 rows, so
+//     bits 0 and 1 of the swizzle differ among 4 rows, and bits 1 to 3 among 8.
 //   * The loads of a round are issued when the registers they go to were just converted, a round ahead of their use.
 // The waves' (m, l, O) are merged through LDS; a sequence with several spans leaves them in the caller's scratch, and
 // the last workgroup of the (sequence, kv head) to finish merges them, by a counter that returns to 0.
@@ -145,6 +179,8 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 __device__ __forceinline__ s16x4_t ds_read_tr(const bf16_t *p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)p);
 }
+
+__device__ __forceinline__ int swizzle(int row) { return (row & 7) | (row & 1) << 3; }
 
 // maximum / sum over the four lanes l % 16 of a wave's 16-lane groups: swap the halves of every 32 lanes, then of 64
 __device__ __forceinline__ float group_max(float x) {
@@ -388,7 +424,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)
                 const int lr = i * 16 + (lane >> 2);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int chunk = ((lane & 3) * 4 + c) ^ ((lr & 7) << 1);
+                    const int chunk = ((lane & 3) * 4 + c) ^ swizzle(lr);
                     *reinterpret_cast<u32x4_t *>(vl + lr * HD + chunk * 8) = kv4_to_bf16(vreg[2 * h + i][c], s2);
                 }
             }
@@ -404,7 +440,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)
             const int tr = rgrp * 4 + (col >> 2);  // this lane's row of a transposed read, in either tile
 #pragma unroll
             for (int db = 0; db < 8; ++db) {
-                const int chunk = (db * 2 + ((col & 3) >> 1)) ^ ((tr & 7) << 1);
+                const int chunk = (db * 2 + ((col & 3) >> 1)) ^ swizzle(tr);
                 const bf16_t *src = vl + tr * HD + chunk * 8 + (col & 1) * 4;
                 const s16x4_t a0 = ds_read_tr(src), a1 = ds_read_tr(src + 16 * HD);
                 o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
@@ -532,19 +568,19 @@ extern "C" size_t hip_kv4_block_bytes(int nkv, int hd, int block_size) {
 extern "C" void hip_store_kv4(const bf16_t *k, const bf16_t *v, const int *slot_mapping, uint8_t *k_cache,
                               uint8_t *v_cache, int T, int nkv, int hd, int block_size) {
     if (T <= 0 || !check_rows("store_kv4", k, v, slot_mapping, k_cache, v_cache, T, nkv, hd, block_size)) return;
-    const long rows = (long)T * nkv;
-    const long blocks = (2 * rows * ROW_LANES + QUANT_THREADS - 1) / QUANT_THREADS;
-    hipLaunchKernelGGL(store_kv4_kernel, dim3((unsigned)blocks), dim3(QUANT_THREADS), 0, g_llmgen_stream, k, v,
-                       slot_mapping, k_cache, v_cache, rows, nkv, block_size);
+    const RowsArgs a = rows_args(slot_mapping, T, nkv, block_size);
+    const int U = rows_a_thread(a.rows);
+    hipLaunchKernelGGL(U == 4 ? store_kv4_kernel<4> : store_kv4_kernel<1>, dim3(row_groups(a.rows, U)), dim3(QUANT_THREADS), 0,
+                       g_llmgen_stream, k, v, k_cache, v_cache, a);
 }
 
 extern "C" void hip_load_kv4(bf16_t *k, bf16_t *v, const int *slot_mapping, const uint8_t *k_cache,
                              const uint8_t *v_cache, int T, int nkv, int hd, int block_size) {
     if (T <= 0 || !check_rows("load_kv4", k, v, slot_mapping, k_cache, v_cache, T, nkv, hd, block_size)) return;
-    const long rows = (long)T * nkv;
-    const long blocks = (2 * rows * ROW_LANES + QUANT_THREADS - 1) / QUANT_THREADS;
-    hipLaunchKernelGGL(load_kv4_kernel, dim3((unsigned)blocks), dim3(QUANT_THREADS), 0, g_llmgen_stream, k, v,
-                       slot_mapping, k_cache, v_cache, rows, nkv, block_size);
+    const RowsArgs a = rows_args(slot_mapping, T, nkv, block_size);
+    const int U = rows_a_thread(a.rows);
+    hipLaunchKernelGGL(U == 4 ? load_kv4_kernel<4> : load_kv4_kernel<1>, dim3(row_groups(a.rows, U)), dim3(QUANT_THREADS), 0,
+                       g_llmgen_stream, k, v, k_cache, v_cache, a);
 }
 
 extern "C" void hip_attn_decode_kv4(bf16_t *out, const bf16_t *q, const uint8_t *k_cache, const uint8_t *v_cache,

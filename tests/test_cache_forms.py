@@ -111,7 +111,7 @@ def test_copies_refuse_pages(capfd, src, dst):
              (ctypes.c_int32 * len(dst))(*dst), len(src))
 
 
-@pytest.mark.parametrize("pool, nbytes, blocks", [(None, 64, 4), (P + 8, 64, 4), (P, 0, 4), (P, 24, 4), (P, 64, 0)])
+@pytest.mark.parametrize("pool, nbytes, blocks", [(None, 64, 4), (P + 8, 64, 4), (P, 0, 4), (P, 24, 4), (P, 64, 0), (P, (1 << 28) + 16, 4)])
 def test_copies_refuse_pools(capfd, pool, nbytes, blocks):
     one = (ctypes.c_int32 * 1)
     _refused(capfd, lib().hip_copy_blocks, (ctypes.c_void_p * 1)(pool), 1, nbytes, blocks, one(0), one(1), 1)
