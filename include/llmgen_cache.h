@@ -58,7 +58,8 @@ void hip_load_kv4(uint16_t *k, uint16_t *v, const int32_t *slot_mapping, const u
  * and NaN among them.
  *
  * out, q [T, nq, hd] bf16; hd == 128, nq / nkv in {1, 2, 4, 8, 16}, scale > 0 and finite.  Softmax statistics and sums
- * are f32; probabilities are rounded to bf16 for the matrix cores.
+ * are f32; probabilities are rounded to bf16 for the matrix cores.  Sums are taken against a running reference and
+ * divided at the end: values of up to 2^96 cannot overflow them, beyond that a result may be infinite.
  *
  * work is the calls' scratch: hip_attn_work_bytes() bytes of device memory (16-byte aligned), set up once by
  * hip_attn_work_init and left ready by every call.  Calls that may run at the same time (two streams, two graphs

@@ -164,6 +164,12 @@ int llmgen_plan_passes(const llmgen_entry *entries, int n_entries, size_t max_to
 void *llmgen_graphs_create(int n_layers, uint16_t *const *k_caches, uint16_t *const *v_caches, int n_head,
                            int n_kv_head, int head_dim, int block_size, size_t max_model_len, int max_seqs,
                            const int *buckets, int n_buckets);
+/* llmgen_graphs_create for layers of another form of the cache (include/llmgen_cache.h): k_caches / v_caches are pools of
+ * that form's pages; form NULL is llmgen_graphs_create.  The graphs keep form's scratch, which their replays share with
+ * whatever else runs on the library's stream.  No reference counterpart. */
+void *llmgen_graphs_create_form(int n_layers, void *const *k_caches, void *const *v_caches, const llmgen_cache_form *form,
+                                int n_head, int n_kv_head, int head_dim, int block_size, size_t max_model_len,
+                                int max_seqs, const int *buckets, int n_buckets);
 /* forward's replay path (executor.zig:541-575): pick the smallest bucket >= n_entries, fill and upload the
  * metadata (one copy), copy the step's q / k / v (device, n_entries rows) into the bucket, replay, copy the
  * first n_entries rows of the output to out_dev.  Asynchronous on the library stream.  Returns the bucket size

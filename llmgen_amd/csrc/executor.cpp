@@ -350,7 +350,8 @@ struct Bucket {
 struct Graphs {
     int n_layers, nq, nkv, hd, block_size, max_blocks;
     size_t max_model_len;
-    std::vector<uint16_t *> kc, vc;
+    std::vector<void *> kc, vc;
+    llmgen_cache_form form{};  // bf16 pages without a window unless set
     std::vector<Bucket> buckets;
     uint8_t *meta_host = nullptr;  // pinned, sized for the largest bucket
     uint64_t step_seed = 0;
@@ -367,7 +368,8 @@ void run_nodes(Graphs &g, Bucket &b, int n_seq) {
     llmgen_step_state st{};
     llmgen_bind_step(&st, b.meta_dev, b.lay, n_seq, n_seq, 0, 1, 0, g.nq, g.nkv, g.hd, g.block_size, g.max_blocks,
                      g.max_model_len, b.part_o, b.part_ml, nullptr, n_seq);
-    for (int l = 0; l < g.n_layers; ++l) llmgen_paged_attention(&st, b.out, b.q, b.k, b.v, g.kc[l], g.vc[l], 1);
+    for (int l = 0; l < g.n_layers; ++l)
+        llmgen_paged_attention_form(&st, &g.form, b.out, b.q, b.k, b.v, g.kc[l], g.vc[l], 1);
 }
 
 void free_bucket(Bucket &b) {
@@ -394,8 +396,16 @@ void llmgen_graphs_destroy(void *graphs) {
 void *llmgen_graphs_create(int n_layers, uint16_t *const *k_caches, uint16_t *const *v_caches, int n_head,
                            int n_kv_head, int head_dim, int block_size, size_t max_model_len, int max_seqs,
                            const int *buckets, int n_buckets) {
+    return llmgen_graphs_create_form(n_layers, reinterpret_cast<void *const *>(k_caches),
+                                     reinterpret_cast<void *const *>(v_caches), nullptr, n_head, n_kv_head, head_dim,
+                                     block_size, max_model_len, max_seqs, buckets, n_buckets);
+}
+
+void *llmgen_graphs_create_form(int n_layers, void *const *k_caches, void *const *v_caches, const llmgen_cache_form *form,
+                                int n_head, int n_kv_head, int head_dim, int block_size, size_t max_model_len,
+                                int max_seqs, const int *buckets, int n_buckets) {
     if (n_layers <= 0 || !k_caches || !v_caches || n_head <= 0 || n_kv_head <= 0 || block_size <= 0 ||
-        max_seqs <= 0)
+        max_seqs <= 0 || (form && (form->window < 0 || form->sinks < 0)))
         return nullptr;
     hipStream_t stream = (hipStream_t)hip_get_stream();
     if (!stream) {
@@ -404,6 +414,7 @@ void *llmgen_graphs_create(int n_layers, uint16_t *const *k_caches, uint16_t *co
     }
     Graphs *g = new Graphs{};
     g->n_layers = n_layers;
+    if (form) g->form = *form;
     g->nq = n_head;
     g->nkv = n_kv_head;
     g->hd = head_dim;

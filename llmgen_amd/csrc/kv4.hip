@@ -129,7 +129,7 @@ bool check_rows(const char *who, const void *k, const void *v, const void *slots
     if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc) & 15)
         return refuse(who, "tensors must be 16-byte aligned");
     if (hd != HD || nkv <= 0 || block_size <= 0) return refuse(who, "unsupported shape (head_dim must be 128)");
-    if ((long)T * nkv >= 1L << 30) return refuse(who, "too many rows");
+    if ((long)T * nkv >= 1L << 29) return refuse(who, "too many rows");
     return true;
 }
 
@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)
             }
         }
         // ---- online softmax of head col.  Once every head has a reference m_run, probabilities are taken against it
-        //      without a maximum (they may exceed 1: o / l is unchanged by a common factor); only a sum beyond 2^64 moves
-        //      the reference ----
+        //      without a maximum (they may exceed 1: o / l is unchanged by a common factor); only a lane's sum beyond
+        //      2^16 moves the reference (so a row's sum stays below 2^31 and values of 2^96 cannot overflow) ----
         u32x2_t p[NT];
         float lsum;
         auto probs = [&](float m_use) {
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)
         bool move = !__all(m_run > -INFINITY);
         if (!move) {
             probs(m_run);
-            move = __any(!(lsum <= 0x1p64f));
+            move = __any(!(lsum <= 0x1p16f));
         }
         if (move) {
             float mx = -INFINITY;

@@ -493,7 +493,7 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
             }
         };
         // Once every row of the wave has a finite reference m_run, the tile's probabilities are taken against it without
-        // a row max (they may exceed 1: o / l is unchanged by the common factor).  Only a row sum beyond 2^64 moves the
+        // a row max (they may exceed 1: o / l is unchanged by the common factor).  Only a row sum beyond 2^16 moves the
         // reference, recomputing the tile against the new row max.
         bool grow = false;
         float m_new = m_run, corr = 1.f;
@@ -506,7 +506,7 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
             probs(m_use);
         } else {
             probs(m_run);
-            if (__any(!(lsum <= 0x1p64f))) {
+            if (__any(!(lsum <= 0x1p16f))) {
                 const float mx = row_max();
                 grow = mx > m_run;
                 m_new = grow ? mx : m_run;

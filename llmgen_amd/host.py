@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import List, Sequence
+from typing import List, Optional, Sequence
 
 import numpy as np
 
@@ -96,6 +96,8 @@ HOST_SIGNATURES = {
                                           ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int), ctypes.c_int]),
     "llmgen_graphs_create": (_P, [ctypes.c_int, ctypes.POINTER(_P), ctypes.POINTER(_P)] + [ctypes.c_int] * 4
                              + [_sz, ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.c_int]),
+    "llmgen_graphs_create_form": (_P, [ctypes.c_int, ctypes.POINTER(_P), ctypes.POINTER(_P), ctypes.POINTER(CacheForm)]
+                                  + [ctypes.c_int] * 4 + [_sz, ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.c_int]),
     "llmgen_graphs_step": (ctypes.c_int, [_P, ctypes.POINTER(Seq), ctypes.POINTER(Entry), ctypes.c_int, _P, _P, _P,
                                           _P]),
     "llmgen_graphs_replay": (ctypes.c_int, [_P]),
@@ -312,16 +314,18 @@ class Blocks:
 
 
 class Graphs:
-    """Decode graph buckets over a list of layers' KV pools (C++: llmgen_graphs_*)."""
+    """Decode graph buckets over a list of layers' KV pools (C++: llmgen_graphs_*).  ``form``: the layers' other form of
+    the cache (:class:`CacheForm`), with the buffer its scratch points into in ``work`` (kept alive here)."""
 
     def __init__(self, k_caches, v_caches, n_head, n_kv_head, head_dim, block_size, max_model_len, max_seqs,
-                 buckets=None):
+                 buckets=None, form: Optional[CacheForm] = None, work=None):
         n = len(k_caches)
         kp = (_P * n)(*[t.data_ptr() for t in k_caches])
         vp = (_P * n)(*[t.data_ptr() for t in v_caches])
         b = None if buckets is None else (ctypes.c_int * len(buckets))(*buckets)
-        self._keep = (k_caches, v_caches)
-        self.h = L().llmgen_graphs_create(n, kp, vp, n_head, n_kv_head, head_dim, block_size, max_model_len,
+        self._keep = (k_caches, v_caches, work)
+        f = None if form is None else ctypes.byref(form)
+        self.h = L().llmgen_graphs_create_form(n, kp, vp, f, n_head, n_kv_head, head_dim, block_size, max_model_len,
                                           max_seqs, b, 0 if buckets is None else len(buckets))
         if not self.h:
             raise RuntimeError("llmgen_graphs_create failed")

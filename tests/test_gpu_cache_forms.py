@@ -466,3 +466,75 @@ def test_model_with_another_form(gpu, kv4, window, sinks):
     if kv4:
         assert page_views(m.kv[0].k, 2, 16)[0].shape == (12, 2, 16, 64)
     _check_error()
+
+
+@pytest.mark.parametrize("kv4, window, sinks", [(True, 0, 0), (True, 90, 4), (False, 90, 4)])
+def test_decode_graph_buckets_of_another_form(gpu, kv4, window, sinks):
+    """The executor's decode graph buckets over layers of such a form, against the eager attention node, with changing
+    batches and pages that the window has passed given back."""
+    _say("buckets", kv4, window)
+    nq, nkv, block, max_len = 8, 4, 16, 512
+    mb = max_len // block
+    work = cache.attn_work()
+    layers = [[], []]
+    mgr = A.PagedAttentionManager()
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    for i in range(2):
+        st = mgr.reserve_layer(i, 100, nkv, block, HD, kv4=kv4, window=window, sinks=sinks, work=work)
+        fill = [torch.randn(100 * block, nkv, HD, generator=gen, device="cuda").to(torch.bfloat16) for _ in range(2)]
+        slots = torch.arange(100 * block, dtype=torch.int32, device="cuda")
+        store = lib().hip_store_kv4 if kv4 else lib().hip_store_kv
+        store(p(fill[0]), p(fill[1]), p(slots), p(st.k), p(st.v), 100 * block, nkv, HD, block)
+        layers[0].append(st.k)
+        layers[1].append(st.v)
+    graphs = host.Graphs(*layers, nq, nkv, HD, block, max_len, 4, form=st.form, work=work)
+    try:
+        rng = np.random.default_rng(0)
+        for n in (1, 3, 4, 2):
+            blocks = host.Blocks(100)
+            lens = [int(x) for x in rng.integers(1, max_len, n)]
+            tables = [blocks.alloc(-(-c // block)) for c in lens]
+            if window:  # pages between the sinks and the window: given back, their entries are not read
+                for c, t in zip(lens, tables):
+                    for j in range(-(-sinks // block), max(0, c - window) // block):
+                        blocks.free([t[j]])
+                        t[j] = 0
+            x = [torch.randn(n, h, HD, generator=gen, device="cuda").to(torch.bfloat16) for h in (nq, nkv, nkv)]
+            entries = [S.Entry(c - 1, 1, t) for c, t in zip(lens, tables)]
+            out = torch.full_like(x[0], 7)
+            seqs = [host.Sequence_([0] * c, t) for c, t in zip(lens, tables)]
+            graphs.step(seqs, [(i, c - 1, 1) for i, c in enumerate(lens)], *x, out)
+            torch.cuda.synchronize()
+            ws = _bind(entries, nq, nkv, block, mb, max_len)
+            eager = torch.full_like(x[0], 7)
+            A.g_attn_mgr = mgr
+            A.PagedAttentionImpl.execute(0, A.AttnNode(eager, x, layer_id=1))  # the bucket's last layer wrote out
+            torch.cuda.synchronize()
+            del ws
+            # buckets are padded to another batch, so the keys may be split otherwise: the last bit of bf16 may differ
+            a, b = out.double().cpu().numpy(), eager.double().cpu().numpy()
+            assert np.isfinite(a).all() and (np.abs(a - b) <= 2.0 ** -7 * np.abs(b) + 2.0 ** -8).all()
+            _check_error()
+    finally:
+        graphs.destroy()
+
+
+def test_large_values_behind_growing_scores(gpu):
+    """Values of the largest size that cannot overflow (2^96), with scores that grow along the context: sums against an
+    early reference stay finite."""
+    for kv4 in (False, True):
+        _say("large values", kv4)
+        s = Step([(700, 1), (500, 90), (90, 90)], 4, 2, 16, kv4, 0, 0, seed=4, poison=False)
+        grow = torch.linspace(0, 3, s.k.shape[0] * 16).view(-1, 1, 16, 1)
+        order = torch.argsort(torch.from_numpy(np.concatenate([s.tables[i][:-(-c // 16)] for i, (c, _) in enumerate(s.spec)]
+                                                              + [[s.bad]])))
+        s.k = (s.k.float() * grow[order]).to(torch.bfloat16)
+        s.v = (s.v.float().clamp(-1, 1) * 2.0 ** 96).to(torch.bfloat16)
+        s.upload()
+        s.prefill(cache.attn_work())
+        s.check("prefill")
+        d = Step([(700, 1)], 4, 2, 16, kv4, 0, 0, seed=4, poison=False)
+        d.k, d.v, d.tables = s.k, s.v, s.tables[:1]
+        d.max_blocks = s.max_blocks
+        d.upload().decode(cache.attn_work())
+        d.check("decode")
