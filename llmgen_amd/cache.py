@@ -24,8 +24,12 @@ def kv4_pool(num_blocks: int, nkv: int, block_size: int, hd: int = 128, device="
 
 
 def attn_work(device="cuda") -> torch.Tensor:
-    """Scratch for the attention calls of one stream, ready for use."""
-    return torch.zeros(lib().hip_attn_work_bytes(), dtype=torch.uint8, device=device)
+    """Scratch for the attention calls of one stream, ready for use there: it is cleared before this returns, as that
+    stream need not be torch's current one (while that is capturing, the graph clears it)."""
+    work = torch.zeros(lib().hip_attn_work_bytes(), dtype=torch.uint8, device=device)
+    if work.is_cuda and not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(work.device).synchronize()
+    return work
 
 
 class BlockCopies:

@@ -91,9 +91,10 @@ inline bool check_attention(const char *who, const void *out, const void *q, con
 
 }  // namespace llmgen_cache
 
-// Internal: the single rows (segments with one query row) of a prefill step over 4-bit pages; defined in kv4.hip,
-// launched by hip_attn_prefill_kv4.  window is NO_WINDOW where there is none.
-__attribute__((visibility("hidden"))) void llmgen_kv4_rows_of_prefill(
+// Internal: the single rows (segments with one query row, `rows` of them as far as the caller knows) of a prefill step
+// over 4-bit pages; defined in kv4.hip, launched by hip_attn_prefill_kv4.  window is NO_WINDOW where there is none.
+// False if the grid would be too large.
+__attribute__((visibility("hidden"))) bool llmgen_kv4_rows_of_prefill(
     bf16_t *out, const bf16_t *q, const uint8_t *k_cache, const uint8_t *v_cache, const int *block_tables,
-    const int *ctx_lens, const int *cu_q, const int *tile_seq, int n_tiles, int nq, int nkv, int max_blocks,
-    int block_size, float scale_log2, int window, int sinks);
+    const int *ctx_lens, const int *cu_q, const int *tile_seq, int n_tiles, int rows, int nq, int nkv, int max_blocks,
+    int block_size, float scale_log2, int window, int sinks, void *work, size_t work_bytes);

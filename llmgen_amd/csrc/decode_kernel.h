@@ -79,6 +79,7 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
         row = cu_q[s];
         if (cu_q[s + 1] - row != 1) return;
     }
+    const int entry = WIN ? by : s;  // whose partials and counters: the list's entry, of which the caller knows the number
     const int ctx_all = WIN ? (int)min((long)ctx_lens[s], (long)max_blocks * block_size) : ctx_lens[s];
     // WIN: visible keys [0, n_sink) and [lo, ctx_all); the window part starts at index n_sink_pad, for key lo4
     int lo = 0, lo4 = 0, n_sink = 0, n_sink_pad = 0;
@@ -476,7 +477,7 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
         if (np == 1) {
             out[((long)row * nq + h) * HD + d] = __builtin_bit_cast(bf16_t, (__bf16)(acc / L));
         } else {
-            const long slot = ((long)s * nq + h) * max_parts + part;
+            const long slot = ((long)entry * nq + h) * max_parts + part;
             if (counters) {  // device-coherent (write-through) stores: read by another workgroup below
                 __hip_atomic_store(part_o + slot * HD + d, acc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 if (d == 0) {
@@ -503,7 +504,7 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
     int &s_last = sm.last;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    int *cnt = counters + (long)s * nkv + kvh;
+    int *cnt = counters + (long)entry * nkv + kvh;
     if (tid == 0) s_last = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == np - 1;
     __syncthreads();
     if (!s_last) return;
@@ -524,7 +525,7 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
     if (staged) {
         for (int i = tid; i < G * np; i += NTH) {
             const int g = i / np, p = i - g * np;
-            const float *ml = part_ml + ((long)s * nq + (long)kvh * G + g) * max_parts * 2 + 2 * p;
+            const float *ml = part_ml + ((long)entry * nq + (long)kvh * G + g) * max_parts * 2 + 2 * p;
             mlb[2 * i] = ld(ml);
             mlb[2 * i + 1] = ld(ml + 1);
         }
@@ -533,8 +534,8 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
     for (int idx = tid; idx < G * HD; idx += NTH) {
         const int g = idx / HD, d = idx % HD;
         const long h = (long)kvh * G + g;
-        const float *ml = part_ml + ((long)s * nq + h) * max_parts * 2;
-        const float *po = part_o + ((long)s * nq + h) * max_parts * HD + d;
+        const float *ml = part_ml + ((long)entry * nq + h) * max_parts * 2;
+        const float *po = part_o + ((long)entry * nq + h) * max_parts * HD + d;
         float M = -INFINITY, num = 0.f, den = 0.f;
         if (np <= MB) {
             float mv[MB], lv[MB], ov[MB];
@@ -579,7 +580,7 @@ __device__ __forceinline__ void decode_split_body(bf16_t *__restrict__ out, floa
                 den += w * ld(ml + 2 * p + 1);
             }
         }
-        out[((long)s * nq + h) * HD + d] = __builtin_bit_cast(bf16_t, (__bf16)(num / den));
+        out[((long)(WIN ? row : s) * nq + h) * HD + d] = __builtin_bit_cast(bf16_t, (__bf16)(num / den));
     }
     if (tid == 0) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }

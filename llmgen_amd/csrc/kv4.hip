@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)
         if (np == 1) {
             out[((long)row * nq + h) * HD + d] = __builtin_bit_cast(bf16_t, (__bf16)(acc / L));
         } else {  // device-coherent stores: another workgroup reads them
-            const long slot = ((long)s * nq + h) * nparts + part;
+            const long slot = ((long)by * nq + h) * nparts + part;
             __hip_atomic_store(part_o + slot * HD + d, acc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (d == 0) {
                 __hip_atomic_store(part_ml + slot * 2, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -497,14 +497,14 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(3)
     //      workgroup elects the last, which reads the partials with device-coherent loads, in span order ----
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    int *cnt = counters + (long)s * nkv + kvh;
+    int *cnt = counters + (long)by * nkv + kvh;
     if (tid == 0) sm.last = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == np - 1;
     __syncthreads();
     if (!sm.last) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     auto ld = [](const float *x) { return __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     float *ml = reinterpret_cast<float *>(sm.v);  // [head][span][m, l]
-    const long slot0 = ((long)s * nq + (long)kvh * G) * nparts;
+    const long slot0 = ((long)by * nq + (long)kvh * G) * nparts;
     for (int i = tid; i < G * np; i += 64 * NW) {
         const int g = i / np, p = i - g * np;
         const float *src = part_ml + (slot0 + (long)g * nparts + p) * 2;
@@ -558,6 +558,39 @@ void launch_decode(bf16_t *out, const bf16_t *q, const uint8_t *kc, const uint8_
     else go(page16 ? attn_decode_kv4_kernel<true, 4> : attn_decode_kv4_kernel<false, 4>);
 }
 
+// The launch over d.S sequences (or entries of a tile list, `rows` of which have a single row), its keys split by this
+// rule; false if the grid would be too large.
+bool launch_split(bf16_t *out, const bf16_t *q, const uint8_t *kc, const uint8_t *vc, const int *bt, const int *ctx,
+                  const int *cu_q, const int *tile_seq, const DecodeShape &d, int rows, int max_ctx, const Work &w) {
+    // How the keys are split, measured over 1 to 200 sequences of 300 to 32768 keys: about 8 waves a CU in all, and as
+    // few spans as that allows, since each span more is one more partial result to merge (32 sequences x 8 heads of 1024
+    // keys: one span of 8 waves 9.4 us, two of 4 waves 18 us).
+    //   * enough (sequence, KV head) pairs for the chip: one span, of 8 waves up to two pairs a CU (256 pairs x 1024
+    //     keys 9.4 us against 11.5 us with 4), of 4 above (512 pairs x 700 keys 11.8 against 14.5 us);
+    //   * fewer pairs: spans of at least one round of their waves; 4 waves, or 8 where that would be more than 8 spans (8
+    //     pairs x 32768 keys: 32 spans of 8 waves 16.0 us, 32 of 4 19.4, 64 of 4 24 us; 8 pairs x 2048 keys: 8 spans of 4
+    //     waves 8.4 us, 4 of 8 9.6 us);
+    //   * at most one round of 8 waves: one span (8 pairs x 512 keys 6.4 us against 7.7 us split).
+    long keys = std::max(1, std::min(max_ctx, d.max_blocks * d.block_size));
+    keys = std::min(keys, (long)d.window + d.sinks + 2 * TILE);
+    const long tiles = (keys + TILE - 1) / TILE, pairs = (long)rows * d.nkv, cus = llmgen_num_cus();
+    int waves = 8;
+    long parts = 1;
+    if (pairs >= 2 * cus) {
+        waves = 4;
+    } else if (pairs < cus && tiles > 8 * NT) {
+        parts = std::min((2 * cus + pairs - 1) / pairs, (tiles + 4 * NT - 1) / (4 * NT));
+        if (parts > 8) parts = (parts + 1) / 2;
+        else waves = 4;
+    }
+    parts = std::min<long>({parts, MAX_PARTS, w.floats / ((long)d.S * d.nq * (HD + 2))});
+    if (parts < 1 || (long)d.S * d.nkv > WORK_COUNTERS) parts = 1;
+    const long span = ((tiles + parts - 1) / parts + NT - 1) / NT * NT;
+    if ((long)d.S * d.nkv * parts > 0x7fffffffL) return false;
+    launch_decode(out, q, kc, vc, bt, ctx, cu_q, tile_seq, d, (int)span, (int)parts, w, waves);
+    return true;
+}
+
 }  // namespace
 
 extern "C" size_t hip_kv4_block_bytes(int nkv, int hd, int block_size) {
@@ -593,43 +626,17 @@ extern "C" void hip_attn_decode_kv4(bf16_t *out, const bf16_t *q, const uint8_t 
         return;
     DecodeShape d{S, nq, nkv, nq / nkv, max_blocks, block_size, scale * LLMGEN_LOG2E,
                   window ? std::min(window, NO_WINDOW) : NO_WINDOW, std::min(sinks, NO_WINDOW)};
-    const Work w = split_work(work, work_bytes);
-    // How the keys are split, measured over 1 to 200 sequences of 300 to 32768 keys: about 8 waves a CU in all, and as
-    // few spans as that allows, since each span more is one more partial result to merge (32 sequences x 8 heads of 1024
-    // keys: one span of 8 waves 9.4 us, two of 4 waves 18 us).
-    //   * enough (sequence, KV head) pairs for the chip: one span, of 8 waves up to two pairs a CU (256 pairs x 1024
-    //     keys 9.4 us against 11.5 us with 4), of 4 above (512 pairs x 700 keys 11.8 against 14.5 us);
-    //   * fewer pairs: spans of at least one round of their waves; 4 waves, or 8 where that would be more than 8 spans (8
-    //     pairs x 32768 keys: 32 spans of 8 waves 16.0 us, 32 of 4 19.4, 64 of 4 24 us; 8 pairs x 2048 keys: 8 spans of 4
-    //     waves 8.4 us, 4 of 8 9.6 us);
-    //   * at most one round of 8 waves: one span (8 pairs x 512 keys 6.4 us against 7.7 us split).
-    long keys = std::max(1, std::min(max_ctx, max_blocks * block_size));
-    keys = std::min(keys, (long)d.window + d.sinks + 2 * TILE);
-    const long tiles = (keys + TILE - 1) / TILE, pairs = (long)S * nkv, cus = llmgen_num_cus();
-    int waves = 8;
-    long parts = 1;
-    if (pairs >= 2 * cus) {
-        waves = 4;
-    } else if (pairs < cus && tiles > 8 * NT) {
-        parts = std::min((2 * cus + pairs - 1) / pairs, (tiles + 4 * NT - 1) / (4 * NT));
-        if (parts > 8) parts = (parts + 1) / 2;
-        else waves = 4;
-    }
-    parts = std::min<long>({parts, MAX_PARTS, w.floats / ((long)S * nq * (HD + 2))});
-    if (parts < 1 || pairs > WORK_COUNTERS) parts = 1;
-    const long span = ((tiles + parts - 1) / parts + NT - 1) / NT * NT;
-    if (pairs * parts > 0x7fffffffL) {
+    if (!launch_split(out, q, k_cache, v_cache, block_tables, ctx_lens, nullptr, nullptr, d, S, max_ctx,
+                      split_work(work, work_bytes)))
         refuse(who, "too many sequences");
-        return;
-    }
-    launch_decode(out, q, k_cache, v_cache, block_tables, ctx_lens, nullptr, nullptr, d, (int)span, (int)parts, w, waves);
 }
 
-// The single rows of a prefill step over 4-bit pages: one workgroup a (row, kv head).
-void llmgen_kv4_rows_of_prefill(bf16_t *out, const bf16_t *q, const uint8_t *k_cache, const uint8_t *v_cache,
+// The single rows of a prefill step over 4-bit pages (`rows` of them, as far as the caller knows).
+bool llmgen_kv4_rows_of_prefill(bf16_t *out, const bf16_t *q, const uint8_t *k_cache, const uint8_t *v_cache,
                                 const int *block_tables, const int *ctx_lens, const int *cu_q, const int *tile_seq,
-                                int n_tiles, int nq, int nkv, int max_blocks, int block_size, float scale_log2, int window,
-                                int sinks) {
+                                int n_tiles, int rows, int nq, int nkv, int max_blocks, int block_size, float scale_log2,
+                                int window, int sinks, void *work, size_t work_bytes) {
     DecodeShape d{n_tiles, nq, nkv, nq / nkv, max_blocks, block_size, scale_log2, window, sinks};
-    launch_decode(out, q, k_cache, v_cache, block_tables, ctx_lens, cu_q, tile_seq, d, 1 << 26, 1, Work{}, 4);
+    return launch_split(out, q, k_cache, v_cache, block_tables, ctx_lens, cu_q, tile_seq, d, rows, max_blocks * block_size,
+                        split_work(work, work_bytes));
 }

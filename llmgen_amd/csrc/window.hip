@@ -13,7 +13,7 @@
 //     order out of the caller's scratch;
 //   * 4-bit pages: a tile's codes are loaded a tile ahead into registers (one 16-byte run of 32 codes of K and one of V
 //     a thread) and converted to bf16 on the way into LDS, so the products and the softmax are the same code;
-//   * single rows of a prefill step are streamed by a decode launch before it.
+//   * single rows of a prefill step are streamed by a decode launch before it, in the same scratch.
 #include "cache_common.h"
 #include "decode_kernel.h"
 #include "hip_common.h"
@@ -39,9 +39,9 @@ struct RowArgs {
     const int *bt, *ctx, *cu_q, *tile_seq;
     int S, nq, nkv, max_blocks, block_size, bs_shift;
     float sl2;
-    int window, sinks, span, nparts;
-    float *part_o, *part_ml;
-    int *counters;
+    int window, sinks, span = 0, nparts = 1;
+    float *part_o = nullptr, *part_ml = nullptr;
+    int *counters = nullptr;
 };
 
 template <int G, int NT, bool POW2, int W>
@@ -71,6 +71,33 @@ void launch_rows_g(const RowArgs &a, int waves) {
         case 8: launch_rows<8, 2, 4>(a); break;
         default: launch_rows<16, 1, 4>(a); break;
     }
+}
+
+// The launch over a.S sequences (or entries of a tile list, `rows` of which have a single row) of up to max_ctx keys;
+// false if the grid would be too large.
+bool launch_split_rows(RowArgs a, int rows, int max_ctx, const Work &w) {
+    const int G = a.nq / a.nkv;
+    // As the decode launch over whole contexts: 8-wave workgroups where the (sequence, KV head) pairs alone nearly fill
+    // the chip, and spans of at least one round of a workgroup's waves, about 8 waves a CU in all.
+    const long pairs = (long)rows * a.nkv;
+    const int waves = G <= 4 && pairs * 2 >= llmgen_num_cus() ? 8 : 4;
+    const int wtok = G >= 16 ? 16 : 32, round = waves * wtok;
+    long keys = std::max(1, std::min(max_ctx, a.max_blocks * a.block_size));
+    keys = std::min(keys, (long)a.window + a.sinks + wtok + 4);
+    const long target = 2L * llmgen_num_cus() * 4 / waves;
+    long parts = std::min<long>({(target + pairs - 1) / pairs, (keys + round - 1) / round, 256,
+                                 w.floats / ((long)a.S * a.nq * (llmgen_decode::HD + 2))});
+    if (parts < 1 || (long)a.S * a.nkv > WORK_COUNTERS) parts = 1;
+    if ((long)a.S * a.nkv * parts > 0x7fffffffL) return false;
+    a.span = (int)(((keys + parts - 1) / parts + wtok - 1) / wtok * wtok);
+    a.nparts = (int)parts;
+    if (parts > 1) {
+        a.part_o = w.part;
+        a.part_ml = w.part + (long)a.S * a.nq * parts * llmgen_decode::HD;
+        a.counters = w.counters;
+    }
+    launch_rows_g(a, waves);
+    return true;
 }
 
 // ------------------------------------------------------------------------------------------------------------
@@ -183,14 +210,19 @@ void prefill(const char *who, bool kv4, bf16_t *out, const bf16_t *q, const void
         return;
     }
     if (single_rows != 0) {
-        if (kv4) {
-            llmgen_kv4_rows_of_prefill(out, q, static_cast<const uint8_t *>(kc), static_cast<const uint8_t *>(vc), bt, ctx,
-                                       cu_q, tile_seq, n_tiles, nq, nkv, max_blocks, block_size, sl2, window, sinks);
-        } else {
-            launch_rows_g(RowArgs{out, q, static_cast<const bf16_t *>(kc), static_cast<const bf16_t *>(vc), bt, ctx, cu_q,
-                                  tile_seq, n_tiles, nq, nkv, max_blocks, block_size, bs_shift, sl2, window, sinks, 64, 1,
-                                  nullptr, nullptr, nullptr},
-                          4);
+        // split as a decode launch's rows are, in the scratch that the second launch uses after it
+        const int known = single_rows > 0 ? rows : n_tiles;
+        const bool ok = kv4 ? llmgen_kv4_rows_of_prefill(out, q, static_cast<const uint8_t *>(kc),
+                                                         static_cast<const uint8_t *>(vc), bt, ctx, cu_q, tile_seq, n_tiles,
+                                                         known, nq, nkv, max_blocks, block_size, sl2, window, sinks, work,
+                                                         work_bytes)
+                            : launch_split_rows(RowArgs{out, q, static_cast<const bf16_t *>(kc),
+                                                        static_cast<const bf16_t *>(vc), bt, ctx, cu_q, tile_seq, n_tiles,
+                                                        nq, nkv, max_blocks, block_size, bs_shift, sl2, window, sinks},
+                                                known, max_blocks * block_size, w);
+        if (!ok) {
+            refuse(who, "too many tiles");
+            return;
         }
     }
     const WindowArgs a{out, q, kc, vc, bt, ctx, cu_q, tile_seq, tile_q0, n_tiles, nq, nkv, G, G / (nw / 2), max_blocks,
@@ -231,32 +263,13 @@ extern "C" void hip_attn_decode_window(bf16_t *out, const bf16_t *q, const bf16_
     if (S <= 0 || !check_attention(who, out, q, k_cache, v_cache, block_tables, ctx_lens, nq, nkv, hd, max_blocks,
                                    block_size, scale, window, sinks, work))
         return;
-    const int G = nq / nkv;
-    const Work w = split_work(work, work_bytes);
-    window = window ? std::min(window, NO_WINDOW) : NO_WINDOW;
-    sinks = std::min(sinks, NO_WINDOW);
-    // As the decode launch over whole contexts: 8-wave workgroups where the (sequence, KV head) pairs alone nearly fill
-    // the chip, and spans of at least one round of a workgroup's waves, about 8 waves a CU in all.
-    const long pairs = (long)S * nkv;
-    const int waves = G <= 4 && pairs * 2 >= llmgen_num_cus() ? 8 : 4;
-    const int wtok = G >= 16 ? 16 : 32, round = waves * wtok;
-    long keys = std::max(1, std::min(max_ctx, max_blocks * block_size));
-    keys = std::min(keys, (long)window + sinks + wtok + 4);
-    const long target = 2L * llmgen_num_cus() * 4 / waves;
-    long parts = std::min<long>({(target + pairs - 1) / pairs, (keys + round - 1) / round, 256,
-                                 w.floats / ((long)S * nq * (llmgen_decode::HD + 2))});
-    if (parts < 1 || pairs > WORK_COUNTERS) parts = 1;
-    if (pairs * parts > 0x7fffffffL) {
+    if (!launch_split_rows(RowArgs{out, q, k_cache, v_cache, block_tables, ctx_lens, nullptr, nullptr, S, nq, nkv,
+                                   max_blocks, block_size,
+                                   (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1,
+                                   scale * LLMGEN_LOG2E, window ? std::min(window, NO_WINDOW) : NO_WINDOW,
+                                   std::min(sinks, NO_WINDOW)},
+                           S, max_ctx, split_work(work, work_bytes)))
         refuse(who, "too many sequences");
-        return;
-    }
-    const long span = ((keys + parts - 1) / parts + wtok - 1) / wtok * wtok;
-    const long rows = (long)S * nq * parts;
-    launch_rows_g(RowArgs{out, q, k_cache, v_cache, block_tables, ctx_lens, nullptr, nullptr, S, nq, nkv, max_blocks,
-                          block_size, (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1,
-                          scale * LLMGEN_LOG2E, window, sinks, (int)span, (int)parts, parts > 1 ? w.part : nullptr,
-                          parts > 1 ? w.part + rows * llmgen_decode::HD : nullptr, w.counters},
-                  waves);
 }
 
 extern "C" void hip_attn_prefill_window(bf16_t *out, const bf16_t *q, const bf16_t *k_cache, const bf16_t *v_cache,

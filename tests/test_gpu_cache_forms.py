@@ -196,6 +196,25 @@ def test_prefill_chunk_behind_long_context(gpu, kv4, nq, nkv, window, sinks):
         assert torch.equal(s.out, first)
 
 
+@pytest.mark.parametrize("kv4", [False, True], ids=["bf16", "kv4"])
+@pytest.mark.parametrize("nq, nkv, block", [(2, 2, 16), (4, 2, 48), (16, 1, 7)])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (2000, 5)])
+def test_prefill_single_rows_of_long_contexts(gpu, kv4, nq, nkv, block, window, sinks):
+    """Single rows whose keys are split over workgroups, behind sequences without rows: more of these than tiles."""
+    _say("prefill long rows", kv4, nq, block, window)
+    spec = [(0, 0)] * 30 + [(3000, 1), (90, 70), (2500, 1), (5, 0), (17, 1), (0, 1), (2049, 1)]
+    s = Step(spec, nq, nkv, block, kv4, window, sinks, seed=nq, max_blocks=-(-9000 // block)).upload()
+    work = cache.attn_work()
+    for single in (5, -1, 1):  # the count, unknown, a wrong one
+        s.out.fill_(7)
+        s.prefill(work, single)
+        s.check(f"single {single}")
+        first = s.out.clone()
+        s.prefill(work, single)
+        assert torch.equal(s.out, first)
+    assert not work[: 4 * nkv * len(spec)].any()  # left ready
+
+
 @pytest.mark.parametrize("G", [1, 2, 4, 8])
 @pytest.mark.parametrize("kv4", [False, True], ids=["bf16", "kv4"])
 def test_prefill_many_units(gpu, kv4, G):
@@ -324,6 +343,22 @@ def test_captured_steps_replay(gpu, kv4):
         torch.cuda.synchronize()
         L.hip_graph_destroy(graph)
     _check_error()
+
+
+def test_scratch_is_ready_for_any_stream(gpu):
+    """Memory that torch's stream still writes when it becomes a scratch is clear for calls on another stream."""
+    _say("scratch ready")
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        dirty = torch.empty(lib().hip_attn_work_bytes(), dtype=torch.uint8, device="cuda")
+        for _ in range(20):
+            dirty.fill_(255)
+        del dirty
+        work = cache.attn_work()
+        with torch.cuda.stream(side):
+            seen = work.clone()
+        side.synchronize()
+        assert not seen.any()
 
 
 def test_two_streams_with_a_scratch_each(gpu):
