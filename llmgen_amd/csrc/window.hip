@@ -109,16 +109,19 @@ constexpr int PIECES_MAX = 16, PIECE_MIN_TILES = 4;
 
 template <int NW, int MODE>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
-    attn_prefill_window_kernel(const llmgen_window::WindowArgs a, int n_units, int P, float *__restrict__ part,
+    attn_prefill_window_kernel(const llmgen_window::WindowArgs a, int n_split, int P, float *__restrict__ part,
                                int *__restrict__ counters) {
     using namespace llmgen_window;
     __shared__ __attribute__((aligned(16))) unsigned char lds[sizeof(WindowLds<NW>)];
     __shared__ int s_last;
-    const int unit = (int)(blockIdx.x % n_units), piece = (int)(blockIdx.x / n_units);
+    // the first n_split units (the last tiles of the list) have P workgroups each, the others one
+    const int bid = (int)blockIdx.x;
+    const bool split = bid < n_split * P;
+    const int unit = split ? bid % n_split : bid - n_split * (P - 1), piece = split ? bid / n_split : 0;
     int pe = 1, j0 = 0, j1 = -1;
     constexpr int PSTRIDE = NW * PART_WAVE_FLOATS;
     float *base = nullptr;
-    if (NW <= 4 && P > 1) {  // which share of the unit's key tiles
+    if (NW <= 4 && split) {  // which share of the unit's key tiles
         const int tile = a.n_tiles - 1 - unit / (a.nkv * a.head_groups);
         const int s = a.tile_seq[tile], q0 = a.tile_q0[tile], q_len = a.cu_q[s + 1] - a.cu_q[s];
         const int ctx = (int)min((long)a.ctx_lens[s], (long)a.max_blocks * a.div.bs);
@@ -152,10 +155,10 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)
 }
 
 template <int NW>
-void launch_prefill(int mode, const llmgen_window::WindowArgs &a, long units, int P, const Work &w) {
+void launch_prefill(int mode, const llmgen_window::WindowArgs &a, long units, long n_split, int P, const Work &w) {
     auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, dim3((unsigned)(units * P)), dim3(64 * NW), 0, g_llmgen_stream, a, (int)units, P, w.part,
-                           w.counters);
+        hipLaunchKernelGGL(kern, dim3((unsigned)(units + n_split * (P - 1))), dim3(64 * NW), 0, g_llmgen_stream, a,
+                           (int)n_split, P, w.part, w.counters);
     };
     using namespace llmgen_window;
     if (mode == KV4) go(attn_prefill_window_kernel<NW, KV4>);
@@ -187,25 +190,29 @@ void prefill(const char *who, bool kv4, bf16_t *out, const bf16_t *q, const void
                                                            : (int)DMA_FLAT;
     // one head a 2-wave workgroup at G = 1, two a 4-wave one, four an 8-wave one
     const Work w = split_work(work, work_bytes);
-    const int rows = std::max(0, std::min(single_rows, n_tiles));  // tiles that leave at once
+    // Single rows leave at once; llmgen_fill_meta puts them first in the list, which the grid walks from its end, so the
+    // units before them are the ones that may be split (in another order, or with a wrong count, other units are: the
+    // result is the same).
+    const int rows = std::max(0, std::min(single_rows, n_tiles)), busy_tiles = n_tiles - rows;
     int nw = G == 1 ? 2 : 4;
-    long units = (long)n_tiles * nkv * (G / (nw / 2)), busy = (long)(n_tiles - rows) * nkv * (G / (nw / 2));
+    long units = (long)n_tiles * nkv * (G / (nw / 2));
+    const long busy = (long)busy_tiles * nkv * (G / (nw / 2));
     const long slots = (long)llmgen_num_cus() * (8 / nw);  // workgroups the chip holds at once
     long P = 1;
-    if (busy > 0 && busy * 2 <= slots && units <= WORK_COUNTERS)
-        P = std::min<long>({PIECES_MAX, slots / busy, w.floats / (units * nw * PART_WAVE_FLOATS)});
+    if (busy > 0 && busy * 2 <= slots && busy <= WORK_COUNTERS)
+        P = std::min<long>({PIECES_MAX, slots / busy, w.floats / (busy * nw * PART_WAVE_FLOATS)});
     if (P < 1) P = 1;
     // Four heads a workgroup read each K/V tile once for all of them, two heads leave two workgroups a CU that hide each
     // other's start and end: 16384 rows x 32 heads with a window of 256 keys 199 -> 169 us with two, of 1024 365 -> 353
     // us, of 4096 432 -> 439 us (pages whose tiles take several DMA descriptors: 192 -> 181, 382 -> 399 us).  Steps of at
     // most one four-head unit a CU want the smaller ones too (a prompt of 2048 tokens 67.7 -> 57.8 us).
     const int short_window = mode == DMA_ROW4 || mode == DMA_FLAT ? 512 : 2048;
-    const long units8 = (long)n_tiles * nkv * (G / 4);
-    if (P == 1 && G >= 4 && window > short_window && units8 > llmgen_num_cus()) {
+    if (P == 1 && G >= 4 && window > short_window && (long)busy_tiles * nkv * (G / 4) > llmgen_num_cus()) {
         nw = 8;
-        units = units8;
+        units = (long)n_tiles * nkv * (G / 4);
     }
-    if (units * P > 0x7fffffffL || (long)n_tiles * nkv > 0x7fffffffL) {
+    const long n_split = P > 1 ? busy : 0;
+    if (units + n_split * (P - 1) > 0x7fffffffL || (long)n_tiles * nkv > 0x7fffffffL) {
         refuse(who, "too many tiles");
         return;
     }
@@ -227,9 +234,9 @@ void prefill(const char *who, bool kv4, bf16_t *out, const bf16_t *q, const void
     }
     const WindowArgs a{out, q, kc, vc, bt, ctx, cu_q, tile_seq, tile_q0, n_tiles, nq, nkv, G, G / (nw / 2), max_blocks,
                        llmgen_cache::page_div(block_size), sl2, window, sinks, single_rows == 0};
-    if (nw == 2) launch_prefill<2>(mode, a, units, (int)P, w);
-    else if (nw == 4) launch_prefill<4>(mode, a, units, (int)P, w);
-    else launch_prefill<8>(mode, a, units, 1, w);
+    if (nw == 2) launch_prefill<2>(mode, a, units, n_split, (int)P, w);
+    else if (nw == 4) launch_prefill<4>(mode, a, units, n_split, (int)P, w);
+    else launch_prefill<8>(mode, a, units, 0, 1, w);
 }
 
 __global__ void __launch_bounds__(256) clear_counters_kernel(int *counters, int n) {
