@@ -71,6 +71,8 @@ class PagedAttentionManager:
         without which long sequences are not split."""
         if window < 0 or sinks < 0:
             raise ValueError("window and sinks must not be negative")
+        if work is not None and not work.is_contiguous():
+            raise ValueError("the scratch must be contiguous")
         if kv4:
             pools = [kv4_pool(num_blocks, nkv, block_size, hd, device) for _ in range(2)]
         else:

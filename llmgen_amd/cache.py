@@ -55,10 +55,19 @@ class BlockCopies:
     def _page_bytes(pool) -> int:
         return pool[0].numel() * pool.element_size()
 
+    @staticmethod
+    def _ids(ids):
+        if getattr(ids, "dtype", None) != np.int32:
+            a = np.asarray(ids)
+            if a.size and (a.dtype.kind not in "iu" or a.min() < -(1 << 31) or a.max() >= 1 << 31):
+                raise ValueError("page ids are whole numbers of 32 bits")
+            ids = a.astype(np.int32)
+        return np.ascontiguousarray(ids)
+
     def run(self, src, dst) -> None:
         """Page src[i] onto page dst[i] in every pool; ids as :meth:`Blocks.compact <llmgen_amd.host.Blocks.compact>`
         returns them (int32 arrays) or any sequences of whole numbers.  The pairs have no order."""
-        src, dst = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
+        src, dst = self._ids(src), self._ids(dst)
         if src.shape != dst.shape or src.ndim != 1:
             raise ValueError("one destination for each source")
         self._call(self._ptrs, len(self.pools), self.page_bytes, self.num_blocks, src.__array_interface__["data"][0],

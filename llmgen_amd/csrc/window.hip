@@ -161,8 +161,10 @@ void launch_prefill(int mode, const llmgen_window::WindowArgs &a, long units, lo
                            (int)n_split, P, w.part, w.counters);
     };
     using namespace llmgen_window;
-    if (mode == KV4) go(attn_prefill_window_kernel<NW, KV4>);
-    else if (mode == DMA_BLOCK) go(attn_prefill_window_kernel<NW, DMA_BLOCK>);
+    if constexpr (NW <= 4) {
+        if (mode == KV4) return go(attn_prefill_window_kernel<NW, KV4>);
+    }
+    if (mode == DMA_BLOCK) go(attn_prefill_window_kernel<NW, DMA_BLOCK>);
     else if (mode == DMA_ROW4) go(attn_prefill_window_kernel<NW, DMA_ROW4>);
     else go(attn_prefill_window_kernel<NW, DMA_FLAT>);
 }
@@ -202,12 +204,13 @@ void prefill(const char *who, bool kv4, bf16_t *out, const bf16_t *q, const void
     if (busy > 0 && busy * 2 <= slots && busy <= WORK_COUNTERS)
         P = std::min<long>({PIECES_MAX, slots / busy, w.floats / (busy * nw * PART_WAVE_FLOATS)});
     if (P < 1) P = 1;
-    // Four heads a workgroup read each K/V tile once for all of them, two heads leave two workgroups a CU that hide each
-    // other's start and end: 16384 rows x 32 heads with a window of 256 keys 199 -> 169 us with two, of 1024 365 -> 353
-    // us, of 4096 432 -> 439 us (pages whose tiles take several DMA descriptors: 192 -> 181, 382 -> 399 us).  Steps of at
-    // most one four-head unit a CU want the smaller ones too (a prompt of 2048 tokens 67.7 -> 57.8 us).
+    // bf16 pages: four heads a workgroup read each K/V tile once for all of them, two heads leave two workgroups a CU that
+    // hide each other's start and end: 16384 rows x 32 heads with a window of 256 keys 186 -> 161 us with two, of 1024
+    // 333 -> 321 us, of 4096 901 -> 922 us (pages whose tiles take several DMA descriptors: 177 -> 167, 342 -> 353 us).
+    // Steps of at most one four-head unit a CU want the smaller ones too (a prompt of 2048 tokens 59.0 -> 51.6 us).  4-bit
+    // pages, whose conversion is shared in the same way, gain more from a second workgroup: 8192 rows 555 -> 532 us.
     const int short_window = mode == DMA_ROW4 || mode == DMA_FLAT ? 512 : 2048;
-    if (P == 1 && G >= 4 && window > short_window && (long)busy_tiles * nkv * (G / 4) > llmgen_num_cus()) {
+    if (!kv4 && P == 1 && G >= 4 && window > short_window && (long)busy_tiles * nkv * (G / 4) > llmgen_num_cus()) {
         nw = 8;
         units = (long)n_tiles * nkv * (G / 4);
     }

@@ -247,7 +247,7 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
     const int drow = lane >> 4, dchunk = lane & 15;
     // 4-bit pages: rows of a tile whose runs a thread takes (4 consecutive threads share a row, 16 take rows 4 apart)
     constexpr int RUN_ROWS = NW == 2 ? 2 : 1;
-    const int run4 = (tid & 255) >> 2, my_run_row = (run4 & ~15) | (run4 & 3) << 2 | (run4 >> 2 & 3);
+    const int run4 = tid >> 2, my_run_row = (run4 & ~15) | (run4 & 3) << 2 | (run4 >> 2 & 3);
     const long hb = llmgen_cache::head_bytes(block_size);
     constexpr bool BY_LANE = MODE == DMA_BLOCK || MODE == DMA_ROW4;
     constexpr int LOOKS = MODE == KV4 ? RUN_ROWS : MODE == DMA_BLOCK ? 1 : LOADS, PER = BY_LANE ? 64 / LOOKS : 1;
@@ -343,11 +343,11 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
     };
 
     // ---- 4-bit pages: a tile is 64 rows x 4 runs of 32 values (16 bytes of codes and a scale byte) of K and of V.  A
-    //      thread takes run tid % 4 of row my_run_row (and of the row 32 further with 128 threads), of both K and V, or
-    //      with 512 threads of one of them.  fetch() loads runs into registers, commit() converts them into a stage
-    constexpr int RUN_KV = NW == 8 ? 1 : 2;
-    u32x4_t run_codes[RUN_ROWS][RUN_KV];
-    uint32_t run_scale[RUN_ROWS][RUN_KV];
+    //      thread takes run tid % 4 of row my_run_row (and of the row 32 further with 128 threads), of both K and V.
+    //      fetch() loads runs into registers, commit() converts them into a stage
+    static_assert(MODE != KV4 || NW <= 4, "256 threads take a tile's runs");
+    u32x4_t run_codes[RUN_ROWS][2];
+    uint32_t run_scale[RUN_ROWS][2];
     auto fetch = [&](int it) {
         const int kb0 = tile_key(it), last = kend - 1 - kb0, run = tid & 3;
         const bool all = (kb0 >= kt.lo || kb0 + BK <= sinks) && last >= BK - 1;  // every row of the tile is read
@@ -360,8 +360,8 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
             const int codes = off * llmgen_cache::CODE_BYTES + run * 16;
             const int scale = block_size * llmgen_cache::CODE_BYTES + off * llmgen_cache::SCALE_BYTES + run;
 #pragma unroll
-            for (int j = 0; j < RUN_KV; ++j) {
-                const uint8_t *p = static_cast<const uint8_t *>((RUN_KV == 1 ? tid >= 256 : j) ? a.vc : a.kc) + at;
+            for (int j = 0; j < 2; ++j) {
+                const uint8_t *p = static_cast<const uint8_t *>(j ? a.vc : a.kc) + at;
                 run_codes[i][j] = ld16(p + codes);
                 run_scale[i][j] = p[scale];
             }
@@ -372,8 +372,8 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
 #pragma unroll
         for (int i = 0; i < RUN_ROWS; ++i)
 #pragma unroll
-            for (int j = 0; j < RUN_KV; ++j) {
-                bf16_t *dst = (RUN_KV == 1 ? tid >= 256 : j) ? Vd : Kd;
+            for (int j = 0; j < 2; ++j) {
+                bf16_t *dst = j ? Vd : Kd;
                 const float sc = llmgen_cache::kv4_scale(run_scale[i][j]);
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
@@ -542,18 +542,12 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
 
     lookup(0);
     if constexpr (MODE == KV4) {
-        // The runs of tile it + 1 were fetched a tile ago; they are converted into the other stage beside the products of
-        // tile it.  Waves 4-7 share a SIMD each with waves 0-3 and convert behind their products, the others before
-        // them, so that one wave's conversions run beside the other's products.
-        const bool early = __builtin_amdgcn_readfirstlane(wave) < 4;
+        // The runs of tile it + 1 were fetched a tile ago; they are converted into the other stage ahead of the products
+        // of tile it, beside those of the CU's other workgroup
         auto turn = [&](int it, const bf16_t *Ks, const bf16_t *Vs, bf16_t *Kn, bf16_t *Vn) {
-            auto next = [&]() {
-                if (it + 1 < n_iter) commit(Kn, Vn);
-                if (it + 2 < n_iter) fetch(it + 2);
-            };
-            if (NW < 8 || early) next();
+            if (it + 1 < n_iter) commit(Kn, Vn);
+            if (it + 2 < n_iter) fetch(it + 2);
             compute(it, Ks, Vs);
-            if (NW == 8 && !early) next();
             __syncthreads();
         };
         fetch(0);

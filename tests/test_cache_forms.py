@@ -129,6 +129,22 @@ def test_block_copies_checks_pools():
         cache.BlockCopies([torch.zeros(4, 64)])
 
 
+def test_block_copies_takes_whole_numbers():
+    ids = cache.BlockCopies._ids
+    for good in ([3, 1], (3, 1), np.array([3, 1]), np.array([3, 1], np.uint8), np.array([3, 9, 1], np.int32)[::2], torch.tensor([3, 1])):
+        a = ids(good)
+        assert a.dtype == np.int32 and a.flags.c_contiguous and a.tolist() == [3, 1]
+    assert ids([]).tolist() == []
+    for bad in ([0.5], [1 << 32], [-(1 << 31) - 1], np.array([1 << 31]), np.array([1.0]), ["1"]):
+        with pytest.raises(ValueError):
+            ids(bad)
+
+
+def test_layer_scratch_is_checked():
+    with pytest.raises(ValueError):
+        A.PagedAttentionManager().reserve_layer(0, 4, 8, 16, 128, device="cpu", window=4, work=torch.zeros(64)[::2])
+
+
 def test_forms_are_checked():
     with pytest.raises(ValueError):
         A.PagedAttentionManager().reserve_layer(0, 4, 8, 16, 128, device="cpu", window=-1)

@@ -291,8 +291,9 @@ def test_block_copies_refuses_other_pools(gpu):
                   torch.zeros(64, 4, dtype=torch.uint8, device="cuda").t(), torch.zeros(4, 65, dtype=torch.uint8, device="cuda")):
         with pytest.raises(ValueError):
             cache.BlockCopies([a, other])
-    with pytest.raises(ValueError):
-        cache.BlockCopies([a]).run([1], [2, 3])
+    for src, dst in (([1], [2, 3]), ([0.5], [1]), ([1 << 32], [1]), (np.array([1 << 32]), [1]), ([[0]], [[1]])):
+        with pytest.raises(ValueError):
+            cache.BlockCopies([a]).run(src, dst)
 
 
 # ------------------------------------------------------------------------------------------ graphs and streams
