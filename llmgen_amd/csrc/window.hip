@@ -9,7 +9,7 @@
 // for masks.
 //   * decode over bf16 pages: the split-K workgroup of decode_kernel.h, walking the visible keys only;
 //   * prefill: the workgroup of window_kernel.h.  A unit is a query tile x KV head x group of NW / 2 heads; with few
-//     units each one's key tiles are split over up to 8 workgroups, whose partial (m, l, O) the last to finish merges in
+//     units each one's key tiles are split over up to 16 workgroups, whose partial (m, l, O) the last to finish merge in
 //     order out of the caller's scratch;
 //   * 4-bit pages: a tile's codes are loaded a tile ahead into registers (one 16-byte run of 32 codes of K and one of V
 //     a thread) and converted to bf16 on the way into LDS, so the products and the softmax are the same code;
@@ -103,9 +103,9 @@ bool launch_split_rows(RowArgs a, int rows, int max_ctx, const Work &w) {
 // ------------------------------------------------------------------------------------------------------------
 // Prefill
 // ------------------------------------------------------------------------------------------------------------
-// Pieces a unit, and key tiles a piece has at least.  Up to 16 pieces: 100 rows behind 8000 keys, 16 units, 48.6 us with
-// 8 and 40.2 us with 16, though the merge reads 68 KB a piece.
-constexpr int PIECES_MAX = 16, PIECE_MIN_TILES = 4;
+// Pieces a unit, and key tiles a piece has at least.  Up to 16 pieces: 100 rows behind 8000 keys, 16 units, 42.5 us
+// with 8 and 33.6 us with 16 on 4-bit pages, 30.0 and 27.0 us on bf16 ones, though the merges read 66 KB a piece.
+constexpr int PIECES_MAX = 16, PIECE_MIN_TILES = 4, UNIT_COUNTERS = 5;  // a counter for each 4 pieces, and for those
 
 template <int NW, int MODE>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
@@ -139,18 +139,28 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)
     float *mine = base ? base + (long)piece * PSTRIDE : nullptr;
     window_body<NW, MODE>(a, unit, lds, j0, j1, mine);
     if constexpr (NW <= 4) {
-        if (pe == 1) return;
-        // publish (device-coherent stores, complete before the barrier), then draw a ticket: the last merges
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (threadIdx.x == 0)
-            s_last = __hip_atomic_fetch_add(counters + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == pe - 1;
-        __syncthreads();
-        if (!s_last) return;
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-        prefill_merge_store_n<PIECES_MAX, NW>(a.out, a.cu_q, a.tile_seq, a.tile_q0, a.n_tiles, a.nq, a.nkv, a.G,
-                                              a.head_groups, unit, base, pe);
-        if (threadIdx.x == 0) __hip_atomic_store(counters + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // The last of the pieces to finish merges them, up to FAN; of more, the last of each 4 neighbours merges these,
+        // and the last of the mergers their results: a CU reads 66 KB a piece (100 rows behind 8000 keys in 16 pieces:
+        // 31.8 us in one go, 26.8 us in two; 64 rows behind 1000 keys in 5 pieces: 18.8 us in one go, 21.5 us in two)
+        int *cnt = counters + unit * UNIT_COUNTERS;
+        const int fan = pe > FAN ? 4 : FAN;
+        for (int at = piece, n = pe, step = 1; n > 1; step *= fan) {
+            // publish (device-coherent stores, complete before the barrier), then draw a ticket
+            const int g = at / fan, first = g * fan, of = min(fan, n - first);
+            float *parts = base + (long)first * step * PSTRIDE;
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            if (threadIdx.x == 0)
+                s_last = __hip_atomic_fetch_add(cnt + g, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of - 1;
+            __syncthreads();
+            if (!s_last) return;
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+            merge_parts<NW>(a, unit, parts, step * PSTRIDE * (int)sizeof(float), of, n > fan ? parts : nullptr);
+            if (threadIdx.x == 0) __hip_atomic_store(cnt + g, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            at = g;
+            n = (n + fan - 1) / fan;
+            cnt += 4;
+        }
     }
 }
 
@@ -201,7 +211,7 @@ void prefill(const char *who, bool kv4, bf16_t *out, const bf16_t *q, const void
     const long busy = (long)busy_tiles * nkv * (G / (nw / 2));
     const long slots = (long)llmgen_num_cus() * (8 / nw);  // workgroups the chip holds at once
     long P = 1;
-    if (busy > 0 && busy * 2 <= slots && busy <= WORK_COUNTERS)
+    if (busy > 0 && busy * 2 <= slots && busy * UNIT_COUNTERS <= WORK_COUNTERS)
         P = std::min<long>({PIECES_MAX, slots / busy, w.floats / (busy * nw * PART_WAVE_FLOATS)});
     if (P < 1) P = 1;
     // bf16 pages: four heads a workgroup read each K/V tile once for all of them, two heads leave two workgroups a CU that

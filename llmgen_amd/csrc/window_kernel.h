@@ -82,6 +82,12 @@ struct WindowArgs {
     bool single;  // segments of one row are computed here (no decode launch for them)
 };
 
+// A partial result: for each wave of the workgroup 16 runs of 64 lanes x 4 values of O -- lane hh * 32 + row, run db * 4 +
+// rr: dims db * 32 + rr * 8 + hh * 4 on -- then m and l of each lane (PART_WAVE_FLOATS in all).  They pass between
+// workgroups while both run, so loads and stores are device-coherent, of 16 bytes a lane (buffer instructions with sc1,
+// as the agent-scope atomics have, which there are for 8 bytes at most).
+constexpr int SC1 = 16;
+
 // One query row (at element `row` of q and out, position pos) over n tiles from j0 on, by one wave: lane = key for the
 // scores, lane = two values of the head for the sums, online softmax in base 2.  Reads only keys that the row sees.  The
 // result goes to out, or as row r of a wave's partial result.
@@ -159,10 +165,11 @@ __device__ __forceinline__ void redo_row(const WindowArgs &a, const int *bt, int
         *reinterpret_cast<uint32_t *>(a.out + row + lane * 2) = pack_bf16x2(o0 / l, o1 / l);
         return;
     }
-    const int d = lane * 2;  // value d of row r lies at [db * 16 + (d / 8) % 4 * 4 + d % 4][half * 32 + r], half = d / 4 % 2
-    float *at = part + ((d >> 5) * 16 + (d >> 3 & 3) * 4 + (d & 3)) * 64 + (d >> 2 & 1) * 32 + r;
+    // values d, d + 1 of row r lie in run (d / 32) * 4 + d / 8 % 4 of lane (d / 4 % 2) * 32 + r, from its d % 4 on
+    const int d = lane * 2;
+    float *at = part + ((d >> 5) * 4 + (d >> 3 & 3)) * 256 + ((d >> 2 & 1) * 32 + r) * 4 + (d & 3);
     __hip_atomic_store(at, o0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(at + 64, o1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(at + 1, o1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (lane < 2) {  // the merge adds the halves' l
         __hip_atomic_store(part + 64 * 64 + lane * 32 + r, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __hip_atomic_store(part + 65 * 64 + lane * 32 + r, lane ? 0.f : l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -171,7 +178,7 @@ __device__ __forceinline__ void redo_row(const WindowArgs &a, const int *bt, int
 
 // The workgroup's work: unit `bid` of the grid (KV head fastest, then group of NW / 2 heads, then tile from the end of
 // the list), key tiles [j0, j1) of it (j1 < 0: to its last).  If part is not null the partial result goes there
-// (device-coherent stores, NW * PART_WAVE_FLOATS floats, the layout prefill_merge_store_n reads) instead of rows to out.
+// (NW * PART_WAVE_FLOATS floats) instead of rows to out.
 //
 // Masking a score does not stop an infinity or NaN in V, as 0 times it is NaN.  Rows whose accumulators end up with one
 // (and whose scores have none: then the result is NaN) are therefore computed again by redo_row, which multiplies only
@@ -610,13 +617,17 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
     const bool mine = row_valid && !(again >> l32 & 1);
 
     if (part) {  // leave the partial result (the merging workgroup reads it with device-coherent loads)
-        float *pw = part + wave * PART_WAVE_FLOATS + lane;
         if (mine || !row_valid) {
+            const __amdgpu_buffer_rsrc_t ps =
+                make_rsrc(reinterpret_cast<const bf16_t *>(part), NW * PART_WAVE_FLOATS * (int)sizeof(float));
+            const int at = wave * PART_WAVE_FLOATS * (int)sizeof(float) + lane * 16;
 #pragma unroll
-            for (int db = 0; db < 4; ++db)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    __hip_atomic_store(pw + (db * 16 + r) * 64, o[db][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int i = 0; i < 16; ++i) {
+                const f32x4_t x = {o[i >> 2][(i & 3) * 4], o[i >> 2][(i & 3) * 4 + 1], o[i >> 2][(i & 3) * 4 + 2],
+                                   o[i >> 2][(i & 3) * 4 + 3]};
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), ps, at, i * 1024, SC1);
+            }
+            float *pw = part + wave * PART_WAVE_FLOATS + lane;
             __hip_atomic_store(pw + 64 * 64, m_run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __hip_atomic_store(pw + 65 * 64, l_run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -637,6 +648,85 @@ __device__ __forceinline__ void window_body(const WindowArgs &a, int bid, unsign
         const int r = __builtin_ctzll(again);
         redo_row<MODE>(a, bt, kvh, ((long)(q_beg + r0 + r) * nq + head) * HD, base_pos + r0 + r, kt, j0, n_iter,
                        part ? part + wave * PART_WAVE_FLOATS : nullptr, r);
+    }
+}
+
+// The sum of np partial results (at most FAN), `stride` bytes apart from base on, of unit `unit`, taken in order: the
+// unit's rows, or (`to` not null) a partial result again.  The loads of one run while the one before it is added.
+constexpr int FAN = 8;
+template <int NW>
+__device__ __forceinline__ void merge_parts(const WindowArgs &a, int unit, const float *base, int stride, int np,
+                                            float *to) {
+    const int kvh = unit % a.nkv, rest = unit / a.nkv, hg = rest % a.head_groups;
+    const int tile = a.n_tiles - 1 - rest / a.head_groups;
+    const int s = a.tile_seq[tile], q0 = a.tile_q0[tile];
+    const int q_beg = a.cu_q[s], q_len = a.cu_q[s + 1] - q_beg;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int head = kvh * a.G + hg * (NW / 2) + (wave >> 1);
+    const int r0 = q0 + (wave & 1) * 32, my_row = r0 + (lane & 31), hh = lane >> 5;
+    if (r0 >= q_len) return;  // an inactive wave left no partial
+    constexpr int PIECE = NW * PART_WAVE_FLOATS * (int)sizeof(float);  // bytes
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(reinterpret_cast<const bf16_t *>(base), (np - 1) * stride + PIECE);
+    const int at = wave * PART_WAVE_FLOATS * (int)sizeof(float);
+    f32x4_t x0[16], x1[16], o[16];
+    auto load = [&](int p, f32x4_t (&x)[16]) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            x[i] = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, at + lane * 16, p * stride + i * 1024, SC1));
+    };
+    load(0, x0);
+    float w[FAN], lv[FAN];
+#pragma unroll
+    for (int p = 0; p < FAN; ++p) {
+        const int pp = min(p, np - 1);  // no branch: pieces past np reread the last one and are not used
+        const uint32_t m = __builtin_amdgcn_raw_buffer_load_b32(rs, at + lane * 4, pp * stride + 64 * 256, SC1);
+        const uint32_t l = __builtin_amdgcn_raw_buffer_load_b32(rs, at + lane * 4, pp * stride + 65 * 256, SC1);
+        w[p] = __builtin_bit_cast(float, m);
+        lv[p] = __builtin_bit_cast(float, l);
+    }
+    float M = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int p = 0; p < FAN; ++p) M = fmaxf(M, w[p]);
+    const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int p = 0; p < FAN; ++p) {
+        w[p] = p < np ? fast_exp2(w[p] - Mu) : 0.f;
+        if (p < np) l += lv[p] * w[p];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    auto add = [&](int p, const f32x4_t (&x)[16]) {
+        float c = 0.f;
+#pragma unroll
+        for (int i = 0; i < FAN; ++i) c = i == p ? w[i] : c;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] += x[i] * c;
+    };
+    for (int p = 0; p < np; p += 2) {
+        if (p + 1 < np) load(p + 1, x1);
+        add(p, x0);
+        if (p + 1 >= np) break;
+        if (p + 2 < np) load(p + 2, x0);
+        add(p + 1, x1);
+    }
+    if (to) {
+        const __amdgpu_buffer_rsrc_t ps = make_rsrc(reinterpret_cast<const bf16_t *>(to), PIECE);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, o[i]), ps, at + lane * 16, i * 1024, SC1);
+        float *pw = to + wave * PART_WAVE_FLOATS + lane;
+        __hip_atomic_store(pw + 64 * 64, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(pw + 65 * 64, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return;
+    }
+    const float l_tot = l + lane_xor(l, 32);
+    if (my_row >= q_len) return;
+    const float inv = 1.f / l_tot;
+    bf16_t *orow = a.out + ((long)(q_beg + my_row) * a.nq + head) * HD + hh * 4;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const f32x4_t y = o[i] * inv;
+        *reinterpret_cast<u32x2_t *>(orow + i * 8) = u32x2_t{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
     }
 }
 

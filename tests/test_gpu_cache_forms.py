@@ -197,6 +197,30 @@ def test_prefill_chunk_behind_long_context(gpu, kv4, nq, nkv, window, sinks):
 
 
 @pytest.mark.parametrize("kv4", [False, True], ids=["bf16", "kv4"])
+@pytest.mark.parametrize("nq, nkv", [(1, 1), (4, 1)])
+def test_prefill_pieces_merged_twice(gpu, kv4, nq, nkv):
+    """Enough key tiles for 16 pieces a unit, 9 of another, and values that rows see or not in some of them."""
+    _say("prefill pieces", kv4, nq)
+    s = Step([(5000, 37), (2200, 66)], nq, nkv, 16, kv4, 0, 0, seed=4)
+    for seq, key, what, dim in ((0, 4970, "v", 3), (0, 1000, "v", 100), (1, 2150, "v", 64), (1, 2170, "k", 1)):
+        x = s.v if what == "v" else s.k
+        x[s.tables[seq][key // 16], 0, key % 16, dim] = float("inf")
+    s.upload()
+    work = cache.attn_work()
+    s.prefill(work, 0)
+    torch.cuda.synchronize()
+    first = s.out.clone()
+    got = s.out.double().cpu().numpy()[:s.rows]
+    ref, tol = s.reference()
+    special = ~np.isfinite(ref)
+    assert special.any() and not special.all()
+    compare(got, ref, tol)
+    s.prefill(work, 0)
+    assert torch.equal(s.out.view(torch.int16), first.view(torch.int16))
+    assert not work[:65536].any()
+
+
+@pytest.mark.parametrize("kv4", [False, True], ids=["bf16", "kv4"])
 @pytest.mark.parametrize("nq, nkv, block", [(2, 2, 16), (4, 2, 48), (16, 1, 7)])
 @pytest.mark.parametrize("window, sinks", [(0, 0), (2000, 5)])
 def test_prefill_single_rows_of_long_contexts(gpu, kv4, nq, nkv, block, window, sinks):
