@@ -86,7 +86,8 @@ void hip_attn_decode_kv4(uint16_t *out, const uint16_t *q, const uint8_t *k_cach
  * keys after this step, tile_seq / tile_q0 [n_tiles] list the query tiles of hip_attn_prefill_tile() rows, in any order
  * (llmgen_fill_meta's is fastest).  Sequences with ctx < q_len are padding: rows of 0; rows behind the last sequence are
  * not written.  single_rows as in hip_attn_prefill_rows: the number of sequences with one row; 0 none, negative
- * unknown.  Single rows are streamed by a decode launch unless the count is 0; a wrong count costs time only. */
+ * unknown.  Single rows are streamed by a decode launch unless the count is 0, their keys split as there; a wrong count
+ * costs time only. */
 void hip_attn_prefill_window(uint16_t *out, const uint16_t *q, const uint16_t *k_cache, const uint16_t *v_cache,
                              const int32_t *block_tables, const int32_t *ctx_lens, const int32_t *cu_q,
                              const int32_t *tile_seq, const int32_t *tile_q0, int n_tiles, int nq, int nkv, int hd,
@@ -102,10 +103,10 @@ void hip_attn_prefill_kv4(uint16_t *out, const uint16_t *q, const uint8_t *k_cac
  * Page copies
  *
  * Copies page src[i] onto page dst[i] in each of n_pools pools (the K and V pools of every layer, of either kind of
- * page).  pools, src and dst are host arrays, read before the call returns: pools holds device pointers (16-byte
- * aligned), the pages are num_blocks x block_bytes (a multiple of 16, at most 2^28).  Every id must lie in [0, num_blocks), no page
- * may be the destination of two pairs, and none both a source and a destination (src[i] == dst[i] is a pair that does
- * nothing): the pairs then have no order.  Otherwise nothing is copied.
+ * page).  pools, src and dst are host arrays, read before the call returns (a captured call keeps what they held): pools
+ * holds device pointers (16-byte aligned), the pages are num_blocks x block_bytes (a multiple of 16, at most 2^28).
+ * Every id must lie in [0, num_blocks), no page may be the destination of two pairs, and none both a source and a
+ * destination (src[i] == dst[i] is a pair that does nothing): the pairs then have no order.  Otherwise nothing is copied.
  * ------------------------------------------------------------------------------------------------------- */
 void hip_copy_blocks(void *const *pools, int n_pools, size_t block_bytes, int num_blocks, const int32_t *src,
                      const int32_t *dst, int n);

@@ -5,7 +5,8 @@
 // Pure HBM copy: the 16-byte pieces of all the launch's pages stand in one row, LOADS of them a thread, so that no thread
 // idles whatever the page size (pages of 1088 bytes 144 -> 74 us against a workgroup a page; of 8704 bytes 206 -> 210 us).
 // A thread's loads are issued before its stores, both past the caches (8704 bytes: 232 -> 210 us).  The pairs have no
-// order (the host refuses chains), so neither do the workgroups.  1096 pages of 8704 bytes in 56 pools: 210 us, 5.1 TB/s.
+// order (the host refuses chains), so neither do the workgroups.  1096 pages of 8704 bytes in 56 pools: 193 to 210 us (box to
+// box), 5.1 to 5.5 TB/s.
 #include "cache_common.h"
 
 #include <algorithm>

@@ -153,13 +153,15 @@ int rows_a_thread(int rows) { return row_groups(rows, 4) >= 4u * llmgen_num_cus(
 //     inner sums are kept to fewer bits: 9e-4 off on dot products of up to 59, where this one is exact to 2e-6.)
 //   * S^T = K Q^T puts the tile's keys in rows (4 a lane) and the group's heads in columns, so the softmax over keys is
 //     lane-local plus two lane exchanges, the running maximum and sum live in the lanes of their head, and two tiles'
-//     probabilities, rounded to bf16 (half a step, 2^-9, as the other attention kernels), are the B fragment of
+//     probabilities, rounded to bf16 (off by at most 2^-8 of each, as in the other attention kernels), are the B fragment of
 //     O^T = V^T P^T as they stand: the fragment's k-slots are assigned to keys in the order the accumulator holds them.
 //   * V: lane l loads bytes 16 l of the tile (key l / 4, run l % 4), converts them and puts the bf16 row into the wave's
 //     8 KB of LDS, from where ds_read_b64_tr_b16 reads it transposed.  Chunks of 16 bytes are swizzled by the row:
 //     writes put 4 rows at once into chunks that differ in bits 2 and 3 only, reads take a pair of chunks of 8 rows, so
 //     bits 0 and 1 of the swizzle differ among 4 rows, and bits 1 to 3 among 8.
 //   * The loads of a round are issued when the registers they go to were just converted, a round ahead of their use.
+// Measured: 16 sequences x 8 KV heads x 32768 keys (571 MB) 92 to 101 us, 5.7 to 6.2 TB/s, the rate of a read-only kernel;
+// 32 ragged sequences of up to 1024 keys (20 MB) 9.2 us, where the chain table -> codes -> products -> merge counts.
 // The waves' (m, l, O) are merged through LDS; a sequence with several spans leaves them in the caller's scratch, and
 // the last workgroup of the (sequence, kv head) to finish merges them, by a counter that returns to 0.
 constexpr int TILE = 16;  // keys a tile

@@ -14,6 +14,10 @@
 //   * 4-bit pages: a tile's codes are loaded a tile ahead into registers (one 16-byte run of 32 codes of K and one of V
 //     a thread) and converted to bf16 on the way into LDS, so the products and the softmax are the same code;
 //   * single rows of a prefill step are streamed by a decode launch before it, in the same scratch.
+// Measured: decode of 64 sequences x 8 KV heads with 4096 visible keys each (1.01 GB) 166 us, 6.1 TB/s; of one sequence
+// with 1000 visible keys 7.7 us, launch, split and merge.  Prefill of 16384 rows x 32 heads with a window of 1024 keys
+// (267 GFLOP) 338 us, 790 TFLOP/s; of 8192 rows x 32 heads on 4-bit pages without one (550 GFLOP) 545 us, 1010 TFLOP/s,
+// bound by the softmax's vector instructions, which the two workgroups of a CU run beside each other's products.
 #include "cache_common.h"
 #include "decode_kernel.h"
 #include "hip_common.h"

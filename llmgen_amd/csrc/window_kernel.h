@@ -672,7 +672,8 @@ __device__ __forceinline__ void merge_parts(const WindowArgs &a, int unit, const
     auto load = [&](int p, f32x4_t (&x)[16]) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            x[i] = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, at + lane * 16, p * stride + i * 1024, SC1));
+            x[i] = __builtin_bit_cast(
+                f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, at + lane * 16, p * stride + i * 1024, SC1));
     };
     load(0, x0);
     float w[FAN], lv[FAN];
