@@ -81,16 +81,42 @@ void launch_rows_g(const RowArgs &a, int waves) {
 // false if the grid would be too large.
 bool launch_split_rows(RowArgs a, int rows, int max_ctx, const Work &w) {
     const int G = a.nq / a.nkv;
-    // As the decode launch over whole contexts: 8-wave workgroups where the (sequence, KV head) pairs alone nearly fill
-    // the chip, and spans of at least one round of a workgroup's waves, about 8 waves a CU in all.
-    const long pairs = (long)rows * a.nkv;
-    const int waves = G <= 4 && pairs * 2 >= llmgen_num_cus() ? 8 : 4;
-    const int wtok = G >= 16 ? 16 : 32, round = waves * wtok;
+    // How the keys are split, measured over 1 to 64 sequences x 8 KV heads of 300 to 8000 visible keys:
+    //   * G = 4, whose 8-wave workgroup fills a CU: always 8 waves, and as many spans as there are CUs for (8 sequences of
+    //     4096 keys: 4 spans of 8 waves 30.7 us, 8 of 4 waves 55 us), but no two of up to 1024 keys in all (16 sequences of
+    //     700 keys: 15.9 us whole, 20.5 us in two);
+    //   * G <= 2: one span for a CU or more a pair, of 8 waves, or of 4 for two pairs a CU (64 sequences of 300 keys 16.3
+    //     and 20.0 us); from half a pair a CU on one of 8 up to 1024 keys (24 sequences of 700: 16.0 us, four of 4 waves
+    //     20.0 us), above that four of 4 (24 of 4096: 68.9 us, one of 8 73.6 us, two of 8 84.9 us); fewer pairs: spans
+    //     of 4 waves, at least a round each, up to 8 of them, or 16 below a quarter of a pair a CU (8 sequences of 4096
+    //     keys: 8 spans 28.2 us, 4 of 8 waves 29.5 us); below an eighth 16 or more of 8 waves where 16 of 4 would be longer
+    //     than a round (one sequence of 8000 keys: 16 of 8 waves 13.9 us, 16 of 4 waves 15.7 us, 64 17.9 us);
+    //   * G >= 8: 4 waves, up to two workgroups a CU, and up to 16 spans (one sequence of 8000 keys: 16 spans 21.8 us, 64
+    //     35 us), one up to 384 keys from a quarter of a pair a CU on (16 sequences of 300: 10.7 us, three 14.6 us).
+    const long pairs = (long)rows * a.nkv, cus = llmgen_num_cus(), wtok = G >= 16 ? 16 : 32;
     long keys = std::max(1, std::min(max_ctx, a.max_blocks * a.block_size));
     keys = std::min(keys, (long)a.window + a.sinks + wtok + 4);
-    const long target = 2L * llmgen_num_cus() * 4 / waves;
-    long parts = std::min<long>({(target + pairs - 1) / pairs, (keys + round - 1) / round, 256,
-                                 w.floats / ((long)a.S * a.nq * (llmgen_decode::HD + 2))});
+    const long rounds4 = (keys + 4 * wtok - 1) / (4 * wtok), rounds8 = (keys + 8 * wtok - 1) / (8 * wtok);
+    int waves = 4;
+    long parts = 1;
+    if (G == 4) {
+        waves = 8;
+        parts = std::min(std::max(cus / pairs, 1L), rounds8);
+        if (parts == 2 && keys <= 1024) parts = 1;
+    } else if (G <= 2) {
+        if (pairs * 2 >= cus) {
+            if (pairs < cus && keys > 1024) parts = 4;
+            else if (pairs < 2 * cus) waves = 8;
+        } else if (pairs * 8 >= cus || rounds4 <= 16) {
+            parts = std::min(rounds4, pairs * 4 >= cus ? 8L : 16L);
+        } else {
+            waves = 8;
+            parts = std::min({rounds8, cus / pairs, std::max(16L, rounds8 / 2)});
+        }
+    } else if (keys > 384 || pairs * 4 < cus) {
+        parts = std::min({(2 * cus + pairs - 1) / pairs, rounds4, std::max(16L, rounds4 / 8)});
+    }
+    parts = std::min<long>({parts, 256, w.floats / ((long)a.S * a.nq * (llmgen_decode::HD + 2))});
     if (parts < 1 || (long)a.S * a.nkv > WORK_COUNTERS) parts = 1;
     if ((long)a.S * a.nkv * parts > 0x7fffffffL) return false;
     a.span = (int)(((keys + parts - 1) / parts + wtok - 1) / wtok * wtok);
