@@ -564,24 +564,28 @@ void launch_decode(bf16_t *out, const bf16_t *q, const uint8_t *kc, const uint8_
 // rule; false if the grid would be too large.
 bool launch_split(bf16_t *out, const bf16_t *q, const uint8_t *kc, const uint8_t *vc, const int *bt, const int *ctx,
                   const int *cu_q, const int *tile_seq, const DecodeShape &d, int rows, int max_ctx, const Work &w) {
-    // How the keys are split, measured over 1 to 200 sequences of 300 to 32768 keys: about 8 waves a CU in all, and as
-    // few spans as that allows, since each span more is one more partial result to merge (32 sequences x 8 heads of 1024
-    // keys: one span of 8 waves 9.4 us, two of 4 waves 18 us).
-    //   * enough (sequence, KV head) pairs for the chip: one span, of 8 waves up to two pairs a CU (256 pairs x 1024
-    //     keys 9.4 us against 11.5 us with 4), of 4 above (512 pairs x 700 keys 11.8 against 14.5 us);
-    //   * fewer pairs: spans of at least one round of their waves; 4 waves, or 8 where that would be more than 8 spans (8
-    //     pairs x 32768 keys: 32 spans of 8 waves 16.0 us, 32 of 4 19.4, 64 of 4 24 us; 8 pairs x 2048 keys: 8 spans of 4
-    //     waves 8.4 us, 4 of 8 9.6 us);
-    //   * at most one round of 8 waves: one span (8 pairs x 512 keys 6.4 us against 7.7 us split).
+    // How the keys are split, measured over 1 to 64 sequences x 8 KV heads of 300 to 32768 keys: as few spans as leave no
+    // CU idle, since each span more is one more partial result to merge.
+    //   * enough (sequence, KV head) pairs for the chip: one span, of 8 waves up to two pairs a CU (256 pairs of 1500 keys
+    //     12.6 us against 15.7 us with 4), of 4 above (512 pairs of 700 keys 11.6 against 14.5 us); from three quarters of
+    //     a pair a CU on (192 pairs of 4096 keys 23.6 us, four spans of 4 waves 26.3 us; 128 pairs 23.2 and 19.5 us);
+    //   * up to two rounds of 8 waves: one span (128 pairs of 700 keys 7.4 us against 12.0 us split, 8 pairs 7.2 and 7.7
+    //     us), or three rounds from three eighths of a pair a CU on (96 pairs of 1500 keys 11.6 and 11.8 us, 64 pairs
+    //     11.0 and 10.6 us);
+    //   * else about two workgroups a CU, the spans a power of two (96 pairs of 4096 keys: 8 spans 16.6 us, 6 17.8 us; 112
+    //     pairs: 4 spans 18.9 us, 8 21.0 us), of at least one round; 4 waves each, or 8 where that would be more than 8 spans (8 pairs of 32768 keys: 32 spans
+    //     of 8 waves 15.8 us, 32 of 4 17.1 us; 8 pairs of 1500 keys: 6 spans of 4 waves 8.2 us, 3 of 8 9.2 us).
     long keys = std::max(1, std::min(max_ctx, d.max_blocks * d.block_size));
     keys = std::min(keys, (long)d.window + d.sinks + 2 * TILE);
     const long tiles = (keys + TILE - 1) / TILE, pairs = (long)rows * d.nkv, cus = llmgen_num_cus();
+    const long rounds = (tiles + 8 * NT - 1) / (8 * NT);  // of 8 waves
     int waves = 8;
     long parts = 1;
     if (pairs >= 2 * cus) {
         waves = 4;
-    } else if (pairs < cus && tiles > 8 * NT) {
-        parts = std::min((2 * cus + pairs - 1) / pairs, (tiles + 4 * NT - 1) / (4 * NT));
+    } else if (pairs * 4 < 3 * cus && rounds > (pairs * 8 >= 3 * cus ? 3 : 2)) {
+        while (2 * parts * pairs <= 3 * cus) parts *= 2;
+        parts = std::min(parts, (tiles + 4 * NT - 1) / (4 * NT));
         if (parts > 8) parts = (parts + 1) / 2;
         else waves = 4;
     }
