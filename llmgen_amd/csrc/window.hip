@@ -9,7 +9,7 @@
 // for masks.
 //   * decode over bf16 pages: the split-K workgroup of decode_kernel.h, walking the visible keys only;
 //   * prefill: the workgroup of window_kernel.h.  A unit is a query tile x KV head x group of NW / 2 heads; with few
-//     units each one's key tiles are split over up to 16 workgroups, whose partial (m, l, O) the last to finish merge in
+//     units each one's key tiles are split over up to 64 workgroups, whose partial (m, l, O) the last to finish merge in
 //     order out of the caller's scratch;
 //   * 4-bit pages: a tile's codes are loaded a tile ahead into registers (one 16-byte run of 32 codes of K and one of V
 //     a thread) and converted to bf16 on the way into LDS, so the products and the softmax are the same code;
@@ -133,9 +133,10 @@ bool launch_split_rows(RowArgs a, int rows, int max_ctx, const Work &w) {
 // ------------------------------------------------------------------------------------------------------------
 // Prefill
 // ------------------------------------------------------------------------------------------------------------
-// Pieces a unit, and key tiles a piece has at least.  Up to 16 pieces: 100 rows behind 8000 keys, 16 units, 42.5 us
-// with 8 and 33.6 us with 16 on 4-bit pages, 30.0 and 27.0 us on bf16 ones, though the merges read 66 KB a piece.
-constexpr int PIECES_MAX = 16, PIECE_MIN_TILES = 4, UNIT_COUNTERS = 5;  // a counter for each 4 pieces, and for those
+// Pieces a unit, and key tiles a piece has at least: 4 up to 16 pieces, 8 beyond.  5 rows behind 32768 keys, 8 units: 70
+// us with 16 pieces and 35.2 us with 64 on 4-bit pages, 73 and 38.4 us on bf16 ones; 100 rows behind 8000 keys, 16 units,
+// 126 tiles: 32.8 us with 16 pieces, 37.1 us with 32, 42.5 us with 8.
+constexpr int PIECES_MAX = 64, PIECE_MIN_TILES = 4, UNIT_COUNTERS = 9;  // a counter for each group of pieces, one for those
 
 template <int NW, int MODE>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)
         const int n = (q_len > 1 || a.single) && ctx >= q_len
                           ? key_tiles(ctx - q_len + q0, ctx - q_len + min(q0 + BQ, q_len), a.window, a.sinks).n
                           : 0;
-        pe = n < 2 ? 1 : min(P, (n + PIECE_MIN_TILES - 1) / PIECE_MIN_TILES);
+        pe = n < 2 ? 1 : min(min(P, (n + PIECE_MIN_TILES - 1) / PIECE_MIN_TILES), max(16, n / 8));
         if (piece >= pe) return;
         if (pe > 1) {
             base = part + (long)unit * P * PSTRIDE;
@@ -169,11 +170,12 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)
     float *mine = base ? base + (long)piece * PSTRIDE : nullptr;
     window_body<NW, MODE>(a, unit, lds, j0, j1, mine);
     if constexpr (NW <= 4) {
-        // The last of the pieces to finish merges them, up to FAN; of more, the last of each 4 neighbours merges these,
-        // and the last of the mergers their results: a CU reads 66 KB a piece (100 rows behind 8000 keys in 16 pieces:
-        // 31.8 us in one go, 26.8 us in two; 64 rows behind 1000 keys in 5 pieces: 18.8 us in one go, 21.5 us in two)
+        // The last of the pieces to finish merges them, up to FAN; of more, the last of each 4 or FAN neighbours merges
+        // these, and the last of the mergers their results: a CU reads 66 KB a piece (100 rows behind 8000 keys in 16
+        // pieces: 31.8 us in one go, 26.8 us in two; 64 rows behind 1000 keys in 5 pieces: 18.8 us in one go, 21.5 us in
+        // two).
         int *cnt = counters + unit * UNIT_COUNTERS;
-        const int fan = pe > FAN ? 4 : FAN;
+        const int fan = pe > FAN && pe <= 16 ? 4 : FAN;
         for (int at = piece, n = pe, step = 1; n > 1; step *= fan) {
             // publish (device-coherent stores, complete before the barrier), then draw a ticket
             const int g = at / fan, first = g * fan, of = min(fan, n - first);
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)
             if (threadIdx.x == 0) __hip_atomic_store(cnt + g, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             at = g;
             n = (n + fan - 1) / fan;
-            cnt += 4;
+            cnt += UNIT_COUNTERS - 1;
         }
     }
 }

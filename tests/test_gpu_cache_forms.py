@@ -199,10 +199,11 @@ def test_prefill_chunk_behind_long_context(gpu, kv4, nq, nkv, window, sinks):
 @pytest.mark.parametrize("kv4", [False, True], ids=["bf16", "kv4"])
 @pytest.mark.parametrize("nq, nkv", [(1, 1), (4, 1)])
 def test_prefill_pieces_merged_twice(gpu, kv4, nq, nkv):
-    """Enough key tiles for 16 pieces a unit, 9 of another, and values that rows see or not in some of them."""
+    """Key tiles for 16 pieces of a unit, 9 of others, 40 of one, and values that rows see or not in some of them."""
     _say("prefill pieces", kv4, nq)
-    s = Step([(5000, 37), (2200, 66)], nq, nkv, 16, kv4, 0, 0, seed=4)
-    for seq, key, what, dim in ((0, 4970, "v", 3), (0, 1000, "v", 100), (1, 2150, "v", 64), (1, 2170, "k", 1)):
+    s = Step([(5000, 37), (2200, 66), (20500, 3)], nq, nkv, 16, kv4, 0, 0, seed=4)
+    for seq, key, what, dim in ((0, 4970, "v", 3), (0, 1000, "v", 100), (1, 2150, "v", 64), (1, 2170, "k", 1),
+                                (2, 20498, "v", 9), (2, 3, "v", 8)):
         x = s.v if what == "v" else s.k
         x[s.tables[seq][key // 16], 0, key % 16, dim] = float("inf")
     s.upload()
