@@ -86,6 +86,13 @@ void hip_qk_norm_rope_store_kv(uint16_t *q_out, uint16_t *k_cache, uint16_t *v_c
                                float eps, const float *cos_tab, const float *sin_tab, const int32_t *positions,
                                const int32_t *slot_mapping, int T, int nq, int nkv, int hd, int block_size);
 
+/* The same into 4-bit pages (llmgen_cache.h): q_out and the pages' bytes are those of hip_rmsnorm + hip_rope +
+ * hip_store_kv4.  Tensors and pools 16-byte aligned.  No reference extern. */
+void hip_qk_norm_rope_store_kv4(uint16_t *q_out, uint8_t *k_cache, uint8_t *v_cache, const uint16_t *q,
+                                const uint16_t *k, const uint16_t *v, const float *q_norm_w, const float *k_norm_w,
+                                float eps, const float *cos_tab, const float *sin_tab, const int32_t *positions,
+                                const int32_t *slot_mapping, int T, int nq, int nkv, int hd, int block_size);
+
 #ifdef __cplusplus
 }
 #endif

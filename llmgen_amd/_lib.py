@@ -70,6 +70,7 @@ SIGNATURES = {
     "hip_sample": (None, [_P, _P, _P, _P, _I, _I, _P]),
     "hip_sample_scratch_bytes": (_SZ, [_I]),
     "hip_qk_norm_rope_store_kv": (None, [_P, _P, _P, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _I, _I, _I, _I, _I]),
+    "hip_qk_norm_rope_store_kv4": (None, [_P, _P, _P, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _I, _I, _I, _I, _I]),
     # include/llmgen_cache.h
     "hip_kv4_block_bytes": (_SZ, [_I, _I, _I]),
     "hip_store_kv4": (None, [_P, _P, _P, _P, _P, _I, _I, _I, _I]),

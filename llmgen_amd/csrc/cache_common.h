@@ -30,6 +30,31 @@ __device__ __forceinline__ u32x4_t kv4_to_bf16(uint32_t w, float scale) {
 // the f32 whose exponent field is scale byte b (0 gives the subnormal field that the conversion reads as 2^-127)
 __device__ __forceinline__ float kv4_scale(uint32_t b) { return __builtin_bit_cast(float, b << 23); }
 
+// Writing: the magnitude bits of the largest of 8 bf16 values (they order as the values do, infinities and NaN above all)
+__device__ __forceinline__ uint32_t kv4_top(u32x4_t x) {
+    const uint32_t x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];
+    return max(max(max(x0 & 0x7fffu, x0 >> 16 & 0x7fffu), max(x1 & 0x7fffu, x1 >> 16 & 0x7fffu)),
+               max(max(x2 & 0x7fffu, x2 >> 16 & 0x7fffu), max(x3 & 0x7fffu, x3 >> 16 & 0x7fffu)));
+}
+// The scale byte of a run whose largest value has the magnitude bits `top`.  floor(log2 amax) is the exponent field for
+// normal numbers.  Subnormal ones have an amax below 2^-126, and e would fall below -127 for any amax under 2^-125: both
+// take the clamp.  Mantissas above 1.75 (0x60 of 7 bits) round up.
+__device__ __forceinline__ int kv4_scale_byte(uint32_t top) {
+    const int byte = (int)(top >> 7) - 2 + ((top & 0x7f) > 0x60 ? 1 : 0);
+    return top >= 0x7f80u ? 255 : top == 0 ? 0 : min(max(byte, 0), 252);
+}
+// 8 bf16 values of a run with that scale byte -> 8 codes
+__device__ __forceinline__ uint32_t kv4_codes(u32x4_t x, int byte) {
+    const uint32_t x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];
+    const float s = kv4_scale(byte == 255 ? 127 : byte);
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x0), s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x1), s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x2), s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x3), s, 3);
+    return byte == 255 ? 0 : w;
+}
+
 // Division of a token's position by the block size: a shift for a power of two, else a multiplication by
 // floor(2^32 / bs), which falls short by at most one for positions below 2^30.
 struct PageDiv {

@@ -72,31 +72,17 @@ __global__ void __launch_bounds__(QUANT_THREADS) store_kv4_kernel(const bf16_t *
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         if (!p[u].live) continue;  // a row's lanes leave together, so the quads below are full
-        const uint32_t x0 = x[u][0], x1 = x[u][1], x2 = x[u][2], x3 = x[u][3];
-        // magnitude bits: they order as the values do, infinities and NaN above all
-        uint32_t top = max(max(max(x0 & 0x7fffu, x0 >> 16 & 0x7fffu), max(x1 & 0x7fffu, x1 >> 16 & 0x7fffu)),
-                           max(max(x2 & 0x7fffu, x2 >> 16 & 0x7fffu), max(x3 & 0x7fffu, x3 >> 16 & 0x7fffu)));
+        uint32_t top = kv4_top(x[u]);
         top = max(top, dpp_u<0xB1>(top));
         top = max(top, dpp_u<0x4E>(top));
-        // floor(log2 amax) is the exponent field for normal numbers.  Subnormal ones have an amax below 2^-126, and e
-        // would fall below -127 for any amax under 2^-125: both take the clamp.  Mantissas above 1.75 (0x60 of 7 bits)
-        // round up.
-        int byte = (int)(top >> 7) - 2 + ((top & 0x7f) > 0x60 ? 1 : 0);
-        byte = top == 0 ? 0 : min(max(byte, 0), 252);
-        const bool bad = top >= 0x7f80u;
-        if (bad) byte = 255;
-        const float s = kv4_scale(bad ? 127 : byte);
-        uint32_t w = 0;
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x0), s, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x1), s, 1);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x2), s, 2);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x3), s, 3);
+        const int byte = kv4_scale_byte(top);
+        const uint32_t w = kv4_codes(x[u], byte);
         // the row's four scale bytes in one word: rotations by 4 and 8 lanes of the 16
         uint32_t scales = (uint32_t)byte << (c >> 2) * 8;
         scales |= dpp_u<0x124>(scales);
         scales |= dpp_u<0x128>(scales);
         uint8_t *pool = p[u].is_v ? vc : kc;
-        *reinterpret_cast<uint32_t *>(pool + p[u].codes + c * 4) = bad ? 0 : w;
+        *reinterpret_cast<uint32_t *>(pool + p[u].codes + c * 4) = w;
         if (c == 0) *reinterpret_cast<uint32_t *>(pool + p[u].scales) = scales;
     }
 }

@@ -208,10 +208,9 @@ class Qwen3:
         token ids (concatenated in entry order).  ``temps[i]`` > 0 samples sequence i (Gumbel-max), else greedy.
         ``seed`` resets the step-seed state (executor.zig:773 advances it every step).  ``fused_qk`` runs a
         layer in nine launches: the projections of one input together (hip_linear3), q/k norm + RoPE + the KV write
-        as one kernel (hip_qk_norm_rope_store_kv), the residual adds with the product before them (hip_linear_add)
-        and SiLU with the product after it (hip_silu_mul); without it the reference graph's launches run one by one.
-        Both give identical values.  4-bit pages have no fused KV write: q/k norm, RoPE and the write are launches of
-        their own."""
+        as one kernel (hip_qk_norm_rope_store_kv, or its form for 4-bit pages), the residual adds with the product before
+        them (hip_linear_add) and SiLU with the product after it (hip_silu_mul); without it the reference graph's launches run one by one.
+        Both give identical values."""
         cfg, L = self.cfg, self.L
         T, S = sum(e.q_len for e in entries), len(entries)
         if len(ids) != T or T > self.max_tokens or S > self.max_seqs:
@@ -260,14 +259,10 @@ class Qwen3:
             if fused_qk:
                 L.hip_linear3(p(q), w("attn_q"), nq * hd, p(k), w("attn_k"), nkv * hd, p(v), w("attn_v"), nkv * hd,
                               p(xn), T, H)
-                if cfg.kv4:
-                    self._norm_rope(q, k, w, g, T)
-                    self._attention(g, i, attn, q, k, v, True)
-                else:
-                    L.hip_qk_norm_rope_store_kv(p(q), p(kv.k), p(kv.v), p(q), p(k), p(v), w("attn_q_norm"),
-                                                w("attn_k_norm"), cfg.rms_eps, p(self.cos), p(self.sin), g.pos, g.slots,
-                                                T, nq, nkv, hd, cfg.block_size)
-                    self._attention(g, i, attn, q, k, v, False)
+                store = L.hip_qk_norm_rope_store_kv4 if cfg.kv4 else L.hip_qk_norm_rope_store_kv
+                store(p(q), p(kv.k), p(kv.v), p(q), p(k), p(v), w("attn_q_norm"), w("attn_k_norm"), cfg.rms_eps,
+                      p(self.cos), p(self.sin), g.pos, g.slots, T, nq, nkv, hd, cfg.block_size)
+                self._attention(g, i, attn, q, k, v, False)
                 L.hip_linear_add(p(x), p(x), p(attn), w("attn_output"), T, H, nq * hd)
                 L.hip_rmsnorm(p(xn), p(x), w("ffn_norm"), T, H, cfg.rms_eps)
                 L.hip_linear3(p(gate), w("ffn_gate"), F, p(up), w("ffn_up"), F, None, None, 0, p(xn), T, H)

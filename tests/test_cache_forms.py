@@ -117,6 +117,17 @@ def test_copies_refuse_pools(capfd, pool, nbytes, blocks):
     _refused(capfd, lib().hip_copy_blocks, (ctypes.c_void_p * 1)(pool), 1, nbytes, blocks, one(0), one(1), 1)
 
 
+@pytest.mark.parametrize("bad", [dict(hd=64), dict(nq=0), dict(nkv=-1), dict(bs=0), dict(kc=P + 8), dict(vc=P + 4), dict(q=P + 2),
+                                 dict(out=P + 8)], ids=str)
+def test_fused_write_refuses(capfd, bad):
+    args = {**dict(out=P, kc=P, vc=P, q=P, k=P, v=P, qw=P, kw=P, eps=1e-6, cos=P, sin=P, pos=P, slots=P, T=1, nq=16, nkv=8, hd=128,
+                   bs=16), **bad}
+    lib().hip_qk_norm_rope_store_kv4(*args.values())
+    assert "hip_qk_norm_rope_store_kv4" in capfd.readouterr().err
+    lib().hip_qk_norm_rope_store_kv4(*{**args, "T": 0}.values())
+    assert not capfd.readouterr().err
+
+
 def test_work_init_refuses(capfd):
     _refused(capfd, lib().hip_attn_work_init, None, 1 << 20)
     _refused(capfd, lib().hip_attn_work_init, P + 4, 1 << 20)

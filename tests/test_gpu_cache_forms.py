@@ -280,6 +280,45 @@ def test_prefill_infinities_between_rows(gpu, kv4, window, sinks, work):
     compare(got, ref, tol)
 
 
+# ------------------------------------------------------------------------------------------ the fused write
+@pytest.mark.parametrize("T, nq, nkv, block", [(1, 1, 1, 16), (5, 16, 8, 16), (300, 32, 8, 256), (33, 3, 3, 7), (64, 8, 1, 48)])
+def test_fused_norm_rope_and_4_bit_write(gpu, T, nq, nkv, block):
+    """One launch leaves the bytes of the five it replaces, at extreme values too; q may be its own output."""
+    from llmgen_amd.qwen3 import rope_tables
+
+    _say("fused write", T, nq, nkv, block)
+    L, gen = lib(), torch.Generator(device="cuda").manual_seed(T)
+    rand = lambda *shape: torch.randn(*shape, generator=gen, device="cuda")  # noqa: E731
+    size = torch.exp(4 * rand(T, 1, 1))
+    q, k, v = ((rand(T, n, HD) * size).to(torch.bfloat16) for n in (nq, nkv, nkv))
+    v[0, 0, :32] = 0
+    v[0, 0, 33], v[-1, -1, 127], k[-1, 0, 5] = float("inf"), float("nan"), float("nan")
+    v[0, 0, 64:96] *= 2.0 ** -126
+    qw, kw = (1 + 0.1 * rand(HD) for _ in range(2))
+    cos, sin = (torch.from_numpy(np.asarray(t, np.float32)).cuda() for t in rope_tables(512, HD, 1e6))
+    pos = torch.randint(0, 512, (T,), generator=gen, device="cuda", dtype=torch.int32)
+    blocks = -(-T // block) + 2
+    slots = torch.randperm(blocks * block, generator=gen, device="cuda")[:T].to(torch.int32)
+    slots[1::7] = -1
+    pools = [torch.full((blocks, L.hip_kv4_block_bytes(nkv, HD, block)), 17, dtype=torch.uint8, device="cuda") for _ in range(6)]
+    qu, ku = q.clone(), k.clone()
+    for x, w, n in ((qu, qw, nq), (ku, kw, nkv)):
+        L.hip_rmsnorm(p(x), p(x), p(w), T * n, HD, 1e-6)
+        L.hip_rope(p(x), p(x), p(cos), p(sin), p(pos), T, n, HD)
+    L.hip_store_kv4(p(ku), p(v), p(slots), p(pools[0]), p(pools[1]), T, nkv, HD, block)
+    qf, qi = torch.empty_like(q), q.clone()
+    for i, (src, dst) in enumerate(((q, qf), (qi, qi))):
+        L.hip_qk_norm_rope_store_kv4(p(dst), p(pools[2 + 2 * i]), p(pools[3 + 2 * i]), p(src), p(k), p(v), p(qw), p(kw), 1e-6,
+                                     p(cos), p(sin), p(pos), p(slots), T, nq, nkv, HD, block)
+    torch.cuda.synchronize()
+    _check_error()
+    for got in (qf, qi):
+        assert torch.equal(got.view(torch.int16), qu.view(torch.int16))
+    for i in (2, 4):
+        assert torch.equal(pools[i], pools[0]) and torch.equal(pools[i + 1], pools[1])
+    assert (pools[0] != 17).any()
+
+
 # ------------------------------------------------------------------------------------------ copies
 @pytest.mark.parametrize("shape, dtype", [((9, 16), torch.uint8), ((40, 3, 1088), torch.uint8), ((12, 2, 16, 128), torch.bfloat16),
                                           ((5, 16400), torch.uint8), ((700, 48), torch.uint8)])
